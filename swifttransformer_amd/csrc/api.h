@@ -121,6 +121,60 @@ int st_gemm_library_allow_workspace(int on);
 int st_sample(int* out, const float* logits, int num_rows, int vocab, const float* temperature,
               const uint32_t* seeds, const uint32_t* draws, hipStream_t stream);
 
+// A token a row from logits and a given random number in [0, 1), after the filters that are given (csrc/sample_filtered.hip).
+// temperature <= 0: the largest logit, lowest index among equals; top_k <= 0, top_p >= 1, min_p <= 0 leave all tokens in.
+int st_sample_filtered(int* out, const float* logits, int64_t row_stride, int num_rows, int vocab, const float* uniforms,
+                       const float* temperature, const int* top_k, const float* top_p, const float* min_p, hipStream_t stream);
+
+// ---- the cache in 8 bits (csrc/quant_cache.hip; the format: csrc/small_float.h): entries [pages, heads, page_size, head_dim] bytes, exponents
+// [pages, heads, page_size] bytes, pages page_stride and exp_stride apart.  Read: results [tokens, heads * head_dim] in the storage type.
+int st_quant_kv_write(void* k_cache, void* v_cache, int64_t page_stride, void* k_exp, void* v_exp, int64_t exp_stride, const void* k_src,
+                      const void* v_src, int64_t src_stride, const int* token_item, const int* positions, const int* block_table, int num_items,
+                      int max_pages, int page_size, int num_pages, int num_tokens, int num_kv_heads, int head_dim, int dtype, hipStream_t stream);
+int st_quant_kv_read(void* k_out, void* v_out, const void* k_cache, const void* v_cache, int64_t page_stride, const void* k_exp,
+                     const void* v_exp, int64_t exp_stride, const int* token_item, const int* positions, const int* block_table, int num_items,
+                     int max_pages, int page_size, int num_pages, int num_tokens, int num_kv_heads, int head_dim, int dtype, hipStream_t stream);
+
+// ---- attention of rows that read the same keys, by tiles (csrc/tile_attention.h).  Which rows:
+//   num_tiles > 0    tiles of tile_rows consecutive rows of items, as st_attn_prefill's
+//   num_groups > 0   every row's keys from row_start[row] on, and for the rows shared_rows[group_off[i] .. group_off[i + 1]) together the
+//                    keys before that, through the block table of the first of them that has a request
+//   else             num_entries rows, row_ids[i] or i, each alone
+// cache_dtype: dtype, or 2 for the 8-bit cache.  Keys in own_splits (and shared_splits) parts; slots is their sum; with more than one,
+// part_o [rows, heads, slots, head_dim] and part_lse [rows, heads, slots] floats (rows: num_rows, or num_entries with row_ids).
+struct StTileAttention {
+    void* out;
+    float* part_o;
+    float* part_lse;
+    const void* q;
+    int64_t q_stride;
+    const void* k_cache;
+    const void* v_cache;
+    int64_t page_stride;
+    const uint8_t* k_exp;
+    const uint8_t* v_exp;
+    int64_t exp_stride;
+    const int* token_item;
+    const int* positions;
+    const int* block_table;
+    const int* row_ids;
+    const int* tile_item;
+    const int* tile_q0;
+    const int* item_tok_off;
+    const int* item_start;
+    const int* item_len;
+    const int* row_start;
+    const int* shared_rows;
+    const int* group_off;
+    int num_rows, num_entries, num_tiles, tile_rows, num_shared, num_groups;
+    int num_items, max_pages, page_size, num_pages;
+    int heads, kv_heads, head_dim;
+    float scale;
+    int own_splits, shared_splits, slots, dtype, cache_dtype;
+    int shared_entries;         // (the library's own)
+};
+int st_tile_attention(const StTileAttention* args, hipStream_t stream);
+
 float st_hash_uniform(uint32_t seed_lo, uint32_t seed_hi, uint32_t draw, uint32_t v);
 
 // ---- short causal convolution over time, one filter a channel (csrc/token_conv.hip)

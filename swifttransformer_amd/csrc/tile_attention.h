@@ -1,0 +1,592 @@
+// Attention of any query rows that read the same keys, on the matrix cores: the kernel behind attention over the 8-bit cache
+// (single tokens, portions of prompts) and attention over shared prefixes.
+//
+// A workgroup takes one key head, up to 16 * RT query rows and a share of the keys.  Query rows are (token, query head of the key head's
+// group) pairs: the heads of one token, of the tokens of a prompt's portion, or of all tokens whose requests begin with the same pages.
+// A key is then read once for all of them.  Its four waves take blocks of 32 keys in turn, each with a running maximum, normaliser and
+// sum of its own (an online softmax in float), and meet in LDS at the end; several workgroups that share a row's keys leave
+// normalised sums and log-sum-exps, which a second kernel joins.
+//
+//   S^T = K Q^T      a lane's scores belong to one query row: l % 16.  Keys come from memory as the operand, eight dims a lane.
+//   O^T += V^T P^T   P^T is the scores' registers as they are.  V goes through LDS, a wave's block in its own part (no barrier), and
+//                    comes back transposed.
+//
+// Keys and values in 8 bits (csrc/small_float.h) become bfloat16 (exact) or float on their way into the product; a key's power of two
+// multiplies its scores, a value's its probability, both without rounding.  Probabilities are rounded to bfloat16 for the second product (at most 2^-8
+// of each, as the queries and keys that they come from are), or stay float in the float instances; maxima, sums and normalisers are float.
+#pragma once
+
+#include "api.h"
+#include "small_float.h"
+
+namespace st {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef int int2v __attribute__((ext_vector_type(2)));
+
+#define ST_LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+// ---- eight elements a lane: as they lie in memory, and as an operand
+template <typename TC> struct Raw8;
+template <> struct Raw8<bf16_t> { uint4 a; };
+template <> struct Raw8<e4m3_t> { uint2 a; };
+template <> struct Raw8<float> { uint4 a, b; };
+
+template <typename TC> __device__ inline Raw8<TC> raw8(const TC* p) { return *reinterpret_cast<const Raw8<TC>*>(p); }
+template <typename TC> __device__ inline void clear(Raw8<TC>& r) { r = Raw8<TC>{}; }
+
+template <typename TQ> struct Op8;
+template <> struct Op8<bf16_t> { bf16x8 v; };
+template <> struct Op8<float> { float v[8]; };
+
+__device__ inline void to_op(const Raw8<bf16_t>& r, Op8<bf16_t>& o) { o.v = __builtin_bit_cast(bf16x8, r.a); }
+__device__ inline void to_op(const Raw8<float>& r, Op8<float>& o) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = __uint_as_float(w[i]);
+}
+__device__ inline void to_op(const Raw8<e4m3_t>& r, Op8<bf16_t>& o) {
+    o.v = __builtin_bit_cast(bf16x8, make_uint4(e4m3x2_to_bf16x2<false>(r.a.x, 1.f), e4m3x2_to_bf16x2<true>(r.a.x, 1.f),
+                                                e4m3x2_to_bf16x2<false>(r.a.y, 1.f), e4m3x2_to_bf16x2<true>(r.a.y, 1.f)));
+}
+__device__ inline void to_op(const Raw8<e4m3_t>& r, Op8<float>& o) {
+    const float2v a = e4m3x2_to_floats<false>(r.a.x), b = e4m3x2_to_floats<true>(r.a.x);
+    const float2v c = e4m3x2_to_floats<false>(r.a.y), d = e4m3x2_to_floats<true>(r.a.y);
+    o.v[0] = a.x; o.v[1] = a.y; o.v[2] = b.x; o.v[3] = b.y; o.v[4] = c.x; o.v[5] = c.y; o.v[6] = d.x; o.v[7] = d.y;
+}
+__device__ inline floatx4 mma8(const Op8<bf16_t>& a, const Op8<bf16_t>& b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ inline floatx4 mma8(const Op8<float>& a, const Op8<float>& b, floatx4 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+}
+__device__ inline void weights_to_op(const float* p, Op8<bf16_t>& o) {
+    o.v = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])));
+}
+__device__ inline void weights_to_op(const float* p, Op8<float>& o) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = p[i];
+}
+
+// ---- a wave's block of 32 values in LDS: rows of kPitch bytes, and an operand of V^T from there: dim 16 * dt + l % 16, keys 4g .. 4g+3 and
+// 16 + 4g .. 16 + 4g+3 (g = l / 16), the keys of the scores that the lane holds
+template <typename TC, int HDP> struct Values {
+    // (a pitch that keeps the rows of a transposing read on different banks)
+    static constexpr int kPitch = 32 * HDP * (int)sizeof(TC) + (sizeof(TC) == 2 ? 32 : 16);
+    static constexpr int kBytes = 32 * kPitch;
+};
+template <int HDP> __device__ inline void value_op(const char* block, int dt, int g, int r16, bf16_t, Op8<bf16_t>& o) {
+    constexpr int P = Values<bf16_t, HDP>::kPitch;
+    const char* at = block + (4 * g + (r16 >> 2)) * P + 32 * dt + 8 * (r16 & 3);
+    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(ST_LDS_PTR(short4v, at)));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(ST_LDS_PTR(short4v, at + 16 * P)));
+    o.v = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
+}
+template <int HDP, typename TQ> __device__ inline void value_op(const char* block, int dt, int g, int r16, e4m3_t, Op8<TQ>& o) {
+    constexpr int P = Values<e4m3_t, HDP>::kPitch;
+    const int k = r16 >> 1;
+    const char* at = block + ((k < 4 ? 4 * g + k : 12 + 4 * g + k)) * P + 16 * dt + 8 * (r16 & 1);
+    Raw8<e4m3_t> r;
+    r.a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(ST_LDS_PTR(int2v, at)));
+    to_op(r, o);
+}
+template <int HDP> __device__ inline void value_op(const char* block, int dt, int g, int r16, float, Op8<float>& o) {
+    constexpr int P = Values<float, HDP>::kPitch;
+    const char* at = block + 4 * g * P + 4 * (16 * dt + r16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = *reinterpret_cast<const float*>(at + ((i & 3) + 16 * (i >> 2)) * P);
+}
+
+// what has been written to LDS by the lanes of a wave is read by others of it: LDS takes a wave's accesses in order, the compiler must too
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
+
+// What a workgroup works on: rows [first, first + count) of the flat list (token j, query head) = (f / group, f % group).
+struct TileWork {
+    int item;              // whose block table
+    int first, count;      // flat rows
+    int lo;                // first key
+    int kind;              // 0 one token, 1 consecutive rows of an item, 2 a list of rows over a prefix
+    int base;              // the token; the item's first batch row; the list's first place
+    int start;             // kind 1: position of the item's first row
+    int slot, splits, split;
+};
+
+// flat row j's token and how many keys it sees; -1 where there is none
+__device__ inline int row_token(const StTileAttention& p, const TileWork& w, int j, int& sees) {
+    int t = w.base + j;
+    if (w.kind == 2) t = p.shared_rows[t];
+    sees = 0;
+    if (t < 0 || t >= p.num_rows) return -1;
+    if (w.kind == 1) {
+        sees = w.start + j + 1;
+    } else {
+        sees = p.positions[t] + 1;
+        if (w.kind == 2) sees = min(sees, p.row_start[t]);
+        if ((uint32_t)p.token_item[t] >= (uint32_t)p.num_items) sees = 0;      // (no request: a padding row)
+    }
+    return t;
+}
+
+template <typename TQ, typename TC, int HDP, int RT>
+__device__ inline void tile_work(const StTileAttention& p, const TileWork& w, int kvh, char* lds) {
+    constexpr int DT = 2 * HDP, R = 16 * RT;
+    constexpr bool QUANT = sizeof(TC) == 1;
+    constexpr int ES = sizeof(TC);
+    constexpr int NV = (2 * HDP * ES + 3) / 4;             // 16-byte chunks of a value that a lane moves (four lanes a value)
+    constexpr int VB = Values<TC, HDP>::kBytes;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, r16 = lane & 15;
+    const int G = p.heads / p.kv_heads, hd = p.head_dim, ps = p.page_size;
+    float* s_m = reinterpret_cast<float*>(lds);             // [4][R] the waves' maxima
+    float* s_l = s_m + 4 * R;                               // [4][R] and normalisers
+    float* s_unit = s_l + 4 * R + wave * 64;                // a wave's keys' and values' powers of two
+    char* s_big = reinterpret_cast<char*>(s_l + 4 * R + (QUANT ? 256 : 0));
+    char* s_v = s_big + wave * VB;                          // [4][32 values], at the end the waves' sums
+
+    // ---- query rows
+    Op8<TQ> qf[RT][HDP];
+    int lim[RT], most = 0, least = 0x7fffffff;
+    const int last_key = p.max_pages * ps;                  // (the host has checked that this is an int)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int f = w.first + 16 * rt + r16;
+        int t = -1, sees = 0, head = 0;
+        if (f < w.count) {
+            const int j = f / G;
+            head = f - j * G;
+            t = row_token(p, w, j, sees);
+        }
+        sees = min(max(sees, 0), last_key);
+        const TQ* row = (const TQ*)p.q + (int64_t)max(t, 0) * p.q_stride + (int64_t)(kvh * G + head) * hd;
+#pragma unroll
+        for (int s = 0; s < HDP; ++s) {
+            const int d = 32 * s + 8 * g;
+            Raw8<TQ> r = raw8(row + (d < hd ? d : 0));
+            if (t < 0 || d >= hd) clear(r);
+            to_op(r, qf[rt][s]);
+        }
+        most = max(most, sees);
+        lim[rt] = t < 0 ? 0x7fffffff : sees;                // (a row that is none takes whatever comes)
+        least = min(least, lim[rt]);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        most = max(most, __shfl_xor(most, o, 64));
+        least = min(least, __shfl_xor(least, o, 64));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+
+    // ---- keys of this workgroup: [kb, ke)
+    const int len = max(most - w.lo, 0);
+    const int blocks = (len + 31) >> 5, share = (blocks + w.splits - 1) / w.splits * 32;
+    const int64_t from = (int64_t)w.lo + (int64_t)w.split * share;
+    const int kb0 = (int)min(from, (int64_t)most), ke = (int)min(from + share, (int64_t)most);
+
+    const bool shifts = (ps & (ps - 1)) == 0;
+    const int page_bits = 31 - __builtin_clz(ps);
+    const int* bt = p.block_table + (int64_t)w.item * p.max_pages;
+    struct Place { int page, row; };
+    const auto look_up = [&](int key) {                     // (a key past the last one stands for that)
+        key = min(key, ke - 1);
+        const int pi = shifts ? key >> page_bits : key / ps;
+        return Place{bt[pi], key - pi * ps};
+    };
+    Raw8<TC> kr[2][HDP];
+    uint4 vr[2][NV];
+    float unit = 0.f;
+    struct Places { Place k[2], v[2], e; };
+    const auto look_up_block = [&](int kb) {
+        Places q;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            q.k[u] = look_up(kb + 16 * u + r16);
+            q.v[u] = look_up(kb + 16 * u + (lane >> 2));
+        }
+        if (QUANT) q.e = look_up(kb + (lane & 31));
+        return q;
+    };
+    uint64_t bad[2];                                        // keys whose page is none of the pool's
+    const auto issue = [&](const Places& q) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool none = (uint32_t)q.k[u].page >= (uint32_t)p.num_pages;
+            bad[u] = __ballot(none);
+            const TC* at = (const TC*)p.k_cache + (uint64_t)(none ? 0u : (uint32_t)q.k[u].page) * (uint64_t)p.page_stride + (kvh * ps + q.k[u].row) * hd;
+#pragma unroll
+            for (int s = 0; s < HDP; ++s) {
+                const int d = 32 * s + 8 * g;
+                kr[u][s] = raw8(at + (d < hd ? d : 0));
+                if (d >= hd) clear(kr[u][s]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool none = (uint32_t)q.v[u].page >= (uint32_t)p.num_pages;
+            const char* at = (const char*)((const TC*)p.v_cache + (uint64_t)(none ? 0u : (uint32_t)q.v[u].page) * (uint64_t)p.page_stride +
+                                           (kvh * ps + q.v[u].row) * hd);
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int b = 16 * (4 * c + (lane & 3));
+                vr[u][c] = *reinterpret_cast<const uint4*>(at + (b < hd * ES ? b : 0));
+                if (none) vr[u][c] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (QUANT) {
+            const bool none = (uint32_t)q.e.page >= (uint32_t)p.num_pages;
+            const uint8_t* e = lane < 32 ? p.k_exp : p.v_exp;
+            const uint32_t field = e[(uint64_t)(none ? 0u : (uint32_t)q.e.page) * (uint64_t)p.exp_stride + kvh * ps + q.e.row];
+            unit = none ? 1.f : __uint_as_float(field << 23);
+        }
+    };
+
+    float m[RT], l[RT];
+    floatx4 acc[RT][DT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = kFloor;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float sl = p.scale * 1.44269504088896340736f;     // scores in units of log2
+
+    int kb = kb0 + 32 * wave;
+    Places next;
+    if (kb < ke) {
+        next = look_up_block(kb);
+        issue(next);
+        next = look_up_block(kb + 128);
+    }
+    for (; kb < ke; kb += 128) {
+        floatx4 sc[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < HDP; ++s)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                Op8<TQ> a;
+                to_op(kr[u][s], a);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
+            }
+        wave_fence();                                       // (the block before has been read)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int b = 16 * (4 * c + (lane & 3));
+                if (b < hd * ES) *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP>::kPitch + b) = vr[u][c];
+            }
+        if (QUANT) s_unit[lane] = unit;
+        const uint64_t bad0 = bad[0], bad1 = bad[1];
+        if (kb + 128 < ke) {
+            issue(next);
+            next = look_up_block(kb + 256);
+        }
+        wave_fence();
+        floatx4 ku[2], vu[2];
+        if (QUANT) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
+                vu[u] = *reinterpret_cast<const floatx4*>(s_unit + 32 + 16 * u + 4 * g);
+            }
+        }
+        const bool whole = kb + 32 <= min(ke, least) && (bad0 | bad1) == 0;
+        Op8<TQ> pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float x[8], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int u = i >> 2, r = i & 3;
+                x[i] = sc[rt][u][r] * sl;
+                if (QUANT) x[i] *= ku[u][r];
+                if (!whole) {
+                    const int key = kb + 16 * u + 4 * g + r;
+                    if (key >= min(ke, lim[rt]) || (((u ? bad1 : bad0) >> (4 * g + r)) & 1)) x[i] = -INFINITY;
+                }
+                top = max_raw(top, x[i]);
+            }
+            top = rows4_max(top);
+            const float mn = max_raw(m[rt], top);
+            if (__any(mn > m[rt])) {
+                const float alpha = __builtin_amdgcn_exp2f(m[rt] - mn);
+                l[rt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+                m[rt] = mn;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - mn);
+                l[rt] += x[i];
+                if (QUANT) x[i] *= vu[i >> 2][i & 3];
+            }
+            weights_to_op(x, pf[rt]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            if (16 * dt < hd) {
+                Op8<TQ> v;
+                value_op<HDP>(s_v, dt, g, r16, TC{}, v);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt], acc[rt][dt]);
+            }
+        }
+    }
+
+    // ---- the waves' results, joined
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = rows4_sum(l[rt]);
+        if (g == 0) {
+            s_m[wave * R + 16 * rt + r16] = m[rt];
+            s_l[wave * R + 16 * rt + r16] = l[rt];
+        }
+    }
+    __syncthreads();                                        // (and all blocks of values have been read)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float top = kFloor;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + 16 * rt + r16]);
+        const float own = __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= own;
+    }
+    // a thread's row and four of its dims, in turns over the subtiles of the head
+    constexpr int JP = 20;                                  // floats between rows of a subtile in LDS
+    float* s_o = reinterpret_cast<float*>(s_big);           // [4][R][JP]
+    const int row = tid >> 2, quad = tid & 3;               // (R <= 64)
+    int t = -1, sees = 0, head = 0;
+    float top = kFloor, sum = 0.f;
+    if (row < R) {
+        const int f = w.first + row;
+        if (f < w.count) {
+            const int j = f / G;
+            head = kvh * G + f - j * G;
+            t = row_token(p, w, j, sees);
+        }
+        for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + row]);
+        for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * __builtin_amdgcn_exp2f(s_m[v * R + row] - top);
+    }
+    // (a sum that is no number belongs to the result)
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t out_row = (int64_t)(w.slot >= 0 ? w.slot : t) * p.heads + head;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        if (16 * dt >= hd) break;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) *reinterpret_cast<floatx4*>(s_o + (wave * R + 16 * rt + r16) * JP + 4 * g) = acc[rt][dt];
+        __syncthreads();
+        if (t >= 0) {
+            floatx4 o = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o += *reinterpret_cast<const floatx4*>(s_o + (v * R + row) * JP + 4 * quad);
+            const float res[4] = {o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse};
+            if (p.slots == 1)
+                Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + 16 * dt + 4 * quad, res);
+            else
+                Elem<float>::store4(p.part_o + (out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split) * hd + 16 * dt + 4 * quad, res);
+        }
+        __syncthreads();
+    }
+    if (t >= 0 && p.slots > 1 && quad == 0)
+        p.part_lse[out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
+// LDS of a workgroup
+template <typename TQ, typename TC, int HDP, int RT>
+constexpr int tile_lds() {
+    return (2 * 4 * 16 * RT + (sizeof(TC) == 1 ? 256 : 0)) * 4 +
+           (4 * Values<TC, HDP>::kBytes > 4 * 16 * RT * 20 * 4 ? 4 * Values<TC, HDP>::kBytes : 4 * 16 * RT * 20 * 4);
+}
+
+// Workgroups: key head fastest (a head's workgroups share its keys and, dealt out in turn, an XCD's L2), then splits, then
+// entries: shared prefixes first (kind 2, RTS subtiles of rows), then single tokens or tiles (RT).
+template <typename TQ, typename TC, int HDP, int RT, int RTS>
+__global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttention p) {
+    extern __shared__ uint4 dyn[];
+    char* lds = reinterpret_cast<char*>(dyn);
+    const int G = p.heads / p.kv_heads;
+    const int kvh = blockIdx.x % p.kv_heads;
+    int y = blockIdx.x / p.kv_heads;
+    TileWork w;
+    w.start = w.lo = 0;
+    w.slot = -1;
+    if (RTS > 0) {
+        if (y < p.shared_entries * p.shared_splits) {
+            int e = y / p.shared_splits;
+            w.split = y - e * p.shared_splits;
+            w.splits = p.shared_splits;
+            w.kind = 2;
+            // the group that entry e belongs to: groups take ceil(rows * G / (16 RTS)) entries each, one behind the other
+            constexpr int R = 16 * RTS;
+            int found = -1, off = 0, n = 0;
+            for (int base = 0; base < p.num_groups && found < 0; base += 64) {
+                const int i = base + (int)(threadIdx.x & 63);
+                int a = 0, b = 0;
+                if (i < p.num_groups) {
+                    a = min(max(p.group_off[i], 0), p.num_shared);
+                    b = min(max(p.group_off[i + 1], a), p.num_shared);
+                }
+                const int mine = ((b - a) * G + R - 1) / R;
+                const int upto = wave_scan(mine);
+                const uint64_t in = __ballot(e < upto);
+                if (in) {
+                    const int at = __ffsll((unsigned long long)in) - 1;
+                    found = base + at;
+                    off = __shfl(a, at, 64);
+                    n = __shfl(b, at, 64) - off;
+                    e -= __shfl(upto - mine, at, 64);
+                } else {
+                    e -= __shfl(upto, 63, 64);
+                }
+            }
+            if (found < 0) return;
+            w.base = __builtin_amdgcn_readfirstlane(off);
+            w.first = __builtin_amdgcn_readfirstlane(e) * R;
+            w.count = __builtin_amdgcn_readfirstlane(n) * G;
+            // the block table: that of the first of the group's rows (of the first 64) that has a request
+            const int i = threadIdx.x & 63;
+            const int t = i < n ? p.shared_rows[w.base + i] : -1;
+            const int item = t >= 0 && t < p.num_rows ? p.token_item[t] : -1;
+            const uint64_t there = __ballot((uint32_t)item < (uint32_t)p.num_items);
+            if (!there) w.lo = 0x7fffffff;                 // none: no key is seen
+            w.item = there ? __builtin_amdgcn_readfirstlane(__shfl(item, __ffsll((unsigned long long)there) - 1, 64)) : 0;
+            tile_work<TQ, TC, HDP, (RTS > 0 ? RTS : 1)>(p, w, kvh, lds);
+            return;
+        }
+        y -= p.shared_entries * p.shared_splits;
+    }
+    const int entry = y / p.own_splits;
+    w.split = y - entry * p.own_splits;
+    w.splits = p.own_splits;
+    constexpr int R = 16 * RT;
+    if (p.num_tiles > 0) {
+        const int chunks = (p.tile_rows * G + R - 1) / R;
+        const int tile = entry / chunks;
+        const int item = p.tile_item[tile], q0 = p.tile_q0[tile];
+        if (item < 0 || item >= p.num_items) return;
+        w.kind = 1;
+        w.item = item;
+        w.base = p.item_tok_off[item] + q0;
+        w.start = p.item_start[item] + q0;
+        w.first = (entry - tile * chunks) * R;
+        w.count = min(p.tile_rows, p.item_len[item] - q0) * G;
+        if (w.first >= w.count) return;
+    } else {
+        const int chunks = (G + R - 1) / R;
+        const int ri = entry / chunks;
+        int t = ri;
+        if (p.row_ids) {
+            t = p.row_ids[ri];
+            if (t < 0 || t >= p.num_rows) return;
+            w.slot = ri;
+        }
+        w.kind = 0;
+        w.base = t;
+        w.first = (entry - ri * chunks) * R;
+        w.count = G;
+        w.item = p.token_item[t];
+        if ((uint32_t)w.item >= (uint32_t)p.num_items) w.item = 0;         // (a padding row sees no key)
+        if (p.row_start) w.lo = max(p.row_start[t], 0);
+    }
+    tile_work<TQ, TC, HDP, RT>(p, w, kvh, lds);
+}
+
+// out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s, w_s = 2^(lse_s - max lse): one wave a row and head
+template <typename TQ>
+__global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p, int rows) {
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, hd = p.head_dim;
+    if (i >= (int64_t)rows * p.heads) return;
+    int64_t ri = i / p.heads;
+    const int64_t head = i - ri * p.heads;
+    int64_t t = ri;
+    if (p.num_tiles > 0) {
+        const int tile = (int)(ri / p.tile_rows), j = (int)(ri - (int64_t)tile * p.tile_rows), item = p.tile_item[tile];
+        if (item < 0 || item >= p.num_items || p.tile_q0[tile] + j >= p.item_len[item]) return;
+        t = ri = p.item_tok_off[item] + p.tile_q0[tile] + j;
+    } else if (p.row_ids) {
+        t = p.row_ids[ri];
+    }
+    if (t < 0 || t >= p.num_rows) return;
+    const int slots = p.row_start && p.row_start[t] <= 0 ? p.own_splits : p.slots;      // (a row of no group has nothing in the others)
+    const int64_t at = (ri * p.heads + head) * p.slots;
+    const float* parts = p.part_o + at * hd;
+    const float lse = lane < slots ? p.part_lse[at + lane] : -INFINITY;
+    const float top = wave_max(lse);
+    const float weight = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
+    const uint64_t held = __ballot(lse != -INFINITY);
+    const float sum = wave_sum(weight);
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    for (int d = lane; d < hd; d += 64) {
+        float o = 0.f;
+        for (int s = 0; s < slots; ++s)
+            if ((held >> s) & 1) o += __shfl(weight, s, 64) * parts[(int64_t)s * hd + d];
+        Elem<TQ>::store((TQ*)p.out + (t * p.heads + head) * hd + d, o * inverse);
+    }
+}
+
+// The instances of a query type: for heads of up to 64, 96, 128 and 256 dims; rows in subtiles of 16: one for single tokens (a
+// group's heads), MAX for tiles and long lists of rows.
+template <typename TQ, typename TC, int HDP, int RT, int RTS>
+int launch_tiles(const StTileAttention& p, hipStream_t stream) {
+    constexpr int lds1 = tile_lds<TQ, TC, HDP, RT>(), lds2 = RTS > 0 ? tile_lds<TQ, TC, HDP, (RTS > 0 ? RTS : 1)>() : 0;
+    const int G = p.heads / p.kv_heads;
+    const int chunks = ((p.num_tiles > 0 ? p.tile_rows : 1) * G + 16 * RT - 1) / (16 * RT);
+    const int64_t entries = (int64_t)(p.num_tiles > 0 ? p.num_tiles : p.num_entries) * chunks;
+    StTileAttention q = p;
+    q.shared_entries = RTS > 0 ? (int)((int64_t)p.num_shared * G / (16 * (RTS > 0 ? RTS : 1))) + p.num_groups : 0;
+    const int64_t groups = (entries * p.own_splits + (int64_t)q.shared_entries * p.shared_splits) * p.kv_heads;
+    ST_CHECK(groups < ((int64_t)1 << 31), "attention: too many rows at once");
+    if (groups == 0) return 0;
+    constexpr int lds = lds1 > lds2 ? lds1 : lds2;
+    if constexpr (lds > 64 * 1024)
+        ST_CHECK(hipFuncSetAttribute((const void*)tile_attention_kernel<TQ, TC, HDP, RT, RTS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
+                 "attention: %d bytes of LDS refused", lds);
+    tile_attention_kernel<TQ, TC, HDP, RT, RTS><<<(unsigned)groups, 256, lds, stream>>>(q);
+    ST_LAUNCH_CHECK("tile_attention");
+    if (p.slots > 1) {
+        const int64_t rows = p.num_tiles > 0 ? (int64_t)p.num_tiles * p.tile_rows : p.num_entries;
+        tile_merge_kernel<TQ><<<(unsigned)((rows * p.heads + 3) / 4), 256, 0, stream>>>(q, (int)rows);
+        ST_LAUNCH_CHECK("tile_merge");
+    }
+    return 0;
+}
+
+template <typename TQ, int HDP, int MAX>
+int launch_tiles_of(const StTileAttention& p, hipStream_t stream) {
+    const bool many = (int64_t)p.num_shared * (p.heads / p.kv_heads) > 16 * (int64_t)p.num_groups;
+    if (p.cache_dtype == 2) {
+        if (p.num_groups > 0) return many ? launch_tiles<TQ, e4m3_t, HDP, 1, MAX>(p, stream) : launch_tiles<TQ, e4m3_t, HDP, 1, 1>(p, stream);
+        return p.num_tiles > 0 ? launch_tiles<TQ, e4m3_t, HDP, MAX, 0>(p, stream) : launch_tiles<TQ, e4m3_t, HDP, 1, 0>(p, stream);
+    }
+    return many ? launch_tiles<TQ, TQ, HDP, 1, MAX>(p, stream) : launch_tiles<TQ, TQ, HDP, 1, 1>(p, stream);
+}
+
+template <typename TQ, int MAX>
+int launch_tiles_by_head(const StTileAttention& p, hipStream_t stream) {
+    if (p.head_dim <= 64) return launch_tiles_of<TQ, 2, MAX>(p, stream);
+    if (p.head_dim <= 96) return launch_tiles_of<TQ, 3, MAX>(p, stream);
+    if (p.head_dim <= 128) return launch_tiles_of<TQ, 4, MAX>(p, stream);
+    return launch_tiles_of<TQ, 8, MAX / 2>(p, stream);
+}
+
+int tile_attention_bf16(const StTileAttention& p, hipStream_t stream);
+int tile_attention_f32(const StTileAttention& p, hipStream_t stream);
+
+}  // namespace st

@@ -70,6 +70,10 @@ def _lib():
         lib.st_probe_fill.argtypes = [_c_p, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p]
         lib.st_probe_mfma.argtypes = [_c_p, _c_int, _c_int, _c_int, _c_p]
         lib.st_sample.argtypes = [_c_p, _c_p, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p]
+        lib.st_sample_filtered.argtypes = [_c_p, _c_p, _c_i64, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]
+        lib.st_quant_kv_write.argtypes = [_c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p] + [_c_int] * 8 + [_c_p]
+        lib.st_quant_kv_read.argtypes = [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p] + [_c_int] * 8 + [_c_p]
+        lib.st_tile_attention.argtypes = [_c_p, _c_p]
         lib.st_token_conv.argtypes = [_c_p, _c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_p]
         lib.st_token_conv_state.argtypes = [_c_p, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int,
@@ -239,6 +243,16 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True) -
         raise KernelError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise KernelError(f"{name} must be contiguous")
+
+
+def _on_one_device(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors that are not all on the current device: the stream is that device's."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"a tensor on {t.device}, the current device is cuda:{here}")
+    if _device_index is not None and _device_index != here:
+        raise KernelError(f"this process launches on cuda:{_device_index}, the current device is cuda:{here}")
 
 
 # ------------------------------------------------------------------------ lookup
@@ -787,6 +801,270 @@ def prefill_available() -> bool:
     return bool(_lib().st_has_attn_prefill())
 
 
+# ------------------------------------------------------------- the cache in 8 bits
+QUANT = torch.float8_e4m3fn      # the entries' type; an entry is worth e4m3 * 2^(exponent - 127)
+
+
+def _quant_cache(k_cache, v_cache, k_exp, v_exp):
+    """Sizes of an 8-bit cache after checking it: (pages, heads, page size, head size, page stride, exponents' page stride)."""
+    if k_cache.dim() != 4:
+        raise KernelError("k_cache must have shape [pages, heads, page size, head size]")
+    num_pages, nkv, ps, hd = k_cache.shape
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _need(c, name, QUANT, (num_pages, nkv, ps, hd), contiguous=False)
+        if c.stride()[1:] != (ps * hd, hd, 1):
+            raise KernelError(f"{name}: a page must be contiguous")
+    for name, e in (("k_exp", k_exp), ("v_exp", v_exp)):
+        _need(e, name, torch.uint8, (num_pages, nkv, ps), contiguous=False)
+        if e.stride()[1:] != (ps, 1):
+            raise KernelError(f"{name}: a page must be contiguous")
+    if k_cache.stride(0) != v_cache.stride(0) or k_exp.stride(0) != v_exp.stride(0):
+        raise KernelError("keys and values must share the page strides")
+    return num_pages, nkv, ps, hd, k_cache.stride(0), k_exp.stride(0)
+
+
+def _d_quant_kv_write(k_cache, v_cache, k_exp, v_exp, k_src, *a, **kw):
+    return {"rows": k_src.shape[0], "width": k_src.shape[1], "bytes": 2 * k_src.numel() * (k_src.element_size() + 1)}
+
+
+@_timed("quant_kv_write", _d_quant_kv_write)
+def quant_kv_write(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, k_src: torch.Tensor,
+                   v_src: torch.Tensor, token_item: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+                   page_size: int) -> None:
+    """Each token's key and value heads into its page of the 8-bit cache.
+
+    k_cache/v_cache: float8_e4m3fn [num_pages, num_kv_heads, page_size, head_dim] views (the page dimension may be strided);
+    k_exp/v_exp: uint8 [num_pages, num_kv_heads, page_size].  A token's head x is stored as e4m3(x * 2^(127 - e)), rounded to nearest even, and e, the
+    smallest exponent with which the largest finite magnitude is at most 448 (127 for a head of zeros).  What is not finite becomes NaN.
+    k_src/v_src: [T, num_kv_heads*head_dim] views with a common row stride, float32 or bfloat16.  A token without an item or a position, or whose page
+    is none of the pool's, is left out; a (item, position) pair may come once in a call."""
+    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+    if ps != page_size:
+        raise KernelError(f"cache pages hold {ps} tokens, the step says {page_size}")
+    T = k_src.shape[0]
+    for name, s in (("k_src", k_src), ("v_src", v_src)):
+        _need(s, name, k_src.dtype, (T, nkv * hd), contiguous=False)
+        if s.stride(1) != 1 or s.stride(0) != k_src.stride(0):
+            raise KernelError(f"{name}: rows must be dense with a common stride")
+    _need(token_item, "token_item", torch.int32, (T,))
+    _need(positions, "positions", torch.int32, (T,))
+    _need_table(block_table)
+    _on_one_device(k_cache, v_cache, k_exp, v_exp, k_src, v_src, token_item, positions, block_table)
+    _check(_lib().st_quant_kv_write(_ptr(k_cache), _ptr(v_cache), stride, _ptr(k_exp), _ptr(v_exp), exp_stride, _ptr(k_src), _ptr(v_src),
+                                    k_src.stride(0) if T > 1 else nkv * hd, _ptr(token_item), _ptr(positions), _ptr(block_table),
+                                    block_table.shape[0], block_table.shape[1], ps, num_pages, T, nkv, hd, dtype_code(k_src.dtype), _stream()))
+
+
+def _need_table(block_table: torch.Tensor) -> None:
+    _need(block_table, "block_table", torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise KernelError("block_table must have shape [items, pages]")
+
+
+def _d_quant_kv_read(k_cache, v_cache, k_exp, v_exp, token_item, positions, block_table, dtype):
+    n = token_item.shape[0] * k_cache.shape[1] * k_cache.shape[3]
+    return {"rows": token_item.shape[0], "width": k_cache.shape[1] * k_cache.shape[3],
+            "bytes": 2 * n * (1 + (2 if dtype == torch.bfloat16 else 4))}
+
+
+@_timed("quant_kv_read", _d_quant_kv_read)
+def quant_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, token_item: torch.Tensor,
+                  positions: torch.Tensor, block_table: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that the 8-bit cache holds for tokens (their items and positions, int32 [T]): two tensors
+    [T, num_kv_heads*head_dim] of ``dtype``, exact in bfloat16 as in float32.  Zeros for a token that ``quant_kv_write`` would leave out."""
+    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+    T = token_item.shape[0]
+    _need(token_item, "token_item", torch.int32, (T,))
+    _need(positions, "positions", torch.int32, (T,))
+    _need_table(block_table)
+    _on_one_device(k_cache, v_cache, k_exp, v_exp, token_item, positions, block_table)
+    code = dtype_code(dtype)
+    k, v = (empty((T, nkv * hd), dtype, k_cache.device) for _ in range(2))
+    _check(_lib().st_quant_kv_read(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), stride, _ptr(k_exp), _ptr(v_exp), exp_stride, _ptr(token_item),
+                                   _ptr(positions), _ptr(block_table), block_table.shape[0], block_table.shape[1], ps, num_pages, T, nkv, hd,
+                                   code, _stream()))
+    return k, v
+
+
+# ------------------------------------------- attention of rows that read the same keys
+class _TileAttention(ctypes.Structure):
+    """Mirror of StTileAttention (csrc/api.h)."""
+    _fields_ = [("out", _c_p), ("part_o", _c_p), ("part_lse", _c_p), ("q", _c_p), ("q_stride", _c_i64), ("k_cache", _c_p), ("v_cache", _c_p),
+                ("page_stride", _c_i64), ("k_exp", _c_p), ("v_exp", _c_p), ("exp_stride", _c_i64), ("token_item", _c_p), ("positions", _c_p),
+                ("block_table", _c_p), ("row_ids", _c_p), ("tile_item", _c_p), ("tile_q0", _c_p), ("item_tok_off", _c_p), ("item_start", _c_p),
+                ("item_len", _c_p), ("row_start", _c_p), ("shared_rows", _c_p), ("group_off", _c_p)] + \
+               [(n, _c_int) for n in ("num_rows", "num_entries", "num_tiles", "tile_rows", "num_shared", "num_groups", "num_items", "max_pages",
+                                      "page_size", "num_pages", "heads", "kv_heads", "head_dim")] + \
+               [("scale", _c_f)] + [(n, _c_int) for n in ("own_splits", "shared_splits", "slots", "dtype", "cache_dtype", "shared_entries")]
+
+
+@functools.lru_cache(maxsize=None)
+def _compute_units(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def tile_splits(workgroups: int, max_keys: int, units: int) -> int:
+    """Parts that the keys are split into, for ``workgroups`` without a split."""
+    return max(1, min(-(-2 * units // max(1, workgroups)), max_keys // 128, 32))
+
+
+def _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, own_splits, shared_splits, out, workspace, **lists):
+    """Checks what all faces of the kernel share and launches it; ``rows``: rows of the partial results."""
+    quant = k_exp is not None
+    if quant:
+        num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+    else:
+        num_pages, nkv, ps, hd = _check_cache(k_cache, v_cache, q)
+        stride, exp_stride = k_cache.stride(0), 0
+    T = q.shape[0]
+    if num_q_heads < 1 or num_q_heads % nkv:
+        raise KernelError(f"{num_q_heads} query heads do not divide into {nkv} key heads")
+    code = dtype_code(q.dtype)
+    _need(q, "q", None, (T, num_q_heads * hd), contiguous=False)
+    if q.stride(1) != 1:
+        raise KernelError("q rows must be dense")
+    _need_table(block_table)
+    slots = own_splits + shared_splits
+    if slots > 64:
+        raise KernelError(f"attention: {slots} parts of the keys (at most 64)")
+    part_o = part_lse = None
+    if slots > 1:
+        n_l = rows * num_q_heads * slots
+        if workspace is None:
+            workspace = empty((n_l * (hd + 1),), torch.float32, q.device)
+        _need(workspace, "workspace", torch.float32)
+        if workspace.numel() < n_l * (hd + 1):
+            raise KernelError("attention workspace is too small")
+        part_o = _ptr(workspace)
+        part_lse = part_o + 4 * n_l * hd
+    _on_one_device(q, k_cache, v_cache, k_exp, v_exp, block_table, out, workspace, *(t for t in lists.values() if isinstance(t, torch.Tensor)))
+    args = _TileAttention(out=_ptr(out), part_o=part_o, part_lse=part_lse, q=_ptr(q), q_stride=q.stride(0) if T > 1 else num_q_heads * hd,
+                          k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), page_stride=stride, k_exp=_ptr(k_exp), v_exp=_ptr(v_exp),
+                          exp_stride=exp_stride, block_table=_ptr(block_table), num_rows=T, num_items=block_table.shape[0],
+                          max_pages=block_table.shape[1], page_size=ps, num_pages=num_pages, heads=num_q_heads, kv_heads=nkv, head_dim=hd,
+                          scale=float(scale), own_splits=own_splits, shared_splits=shared_splits, slots=slots, dtype=code,
+                          cache_dtype=2 if quant else code,
+                          **{n: _ptr(t) if isinstance(t, torch.Tensor) else t for n, t in lists.items() if t is not None})
+    _check(_lib().st_tile_attention(ctypes.byref(args), _stream()))
+    return out
+
+
+def _tile_out(q, out, width):
+    if out is None:
+        out = empty((q.shape[0], width), q.dtype, q.device)
+    _need(out, "out", q.dtype, (q.shape[0], width))
+    return out
+
+
+def _key_bound(max_keys: int, block_table: torch.Tensor, page_size: int) -> int:
+    most = block_table.shape[-1] * page_size
+    return most if max_keys <= 0 else min(int(max_keys), most)
+
+
+def _d_attention_quant(q, k_cache, v_cache, k_exp, v_exp, *a, **kw):
+    return {"rows": q.shape[0], "heads": q.shape[1] // k_cache.shape[3], "kv_heads": k_cache.shape[1], "head_dim": k_cache.shape[3], "elem": 1}
+
+
+@_timed("attention_rows_quant", _d_attention_quant)
+def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+                         token_item: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor, num_q_heads: int, scale: float, *,
+                         max_keys: int = 0, num_splits: int = 0, row_ids: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_rows`` over the 8-bit cache (``quant_kv_write``): each query row attends over its request's cached keys [0, position].
+
+    q: [T, num_q_heads*head_dim] view (row stride free), float32 or bfloat16.  Returns [T, num_q_heads*head_dim]; with ``row_ids`` (entries of -1
+    are skipped) only those batch rows are computed and written.  A row without an item or a position gets zeros.  ``max_keys``: the most keys that
+    a row reads, for the choice of ``num_splits`` where that is 0 (default: what the block table can hold); results do not need it to
+    be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 1)."""
+    T, hd = q.shape[0], k_cache.shape[-1]
+    _need(token_item, "token_item", torch.int32, (T,))
+    _need(positions, "positions", torch.int32, (T,))
+    if row_ids is not None:
+        _need(row_ids, "row_ids", torch.int32, (row_ids.shape[0],))
+    rows = T if row_ids is None else row_ids.shape[0]
+    out = _tile_out(q, out, num_q_heads * hd)
+    if rows == 0:
+        return out
+    if num_splits <= 0:
+        num_splits = tile_splits(rows * k_cache.shape[1], _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(q.device.index))
+    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, int(num_splits), 0, out, workspace,
+                           token_item=token_item, positions=positions, row_ids=row_ids, num_entries=rows)
+
+
+@_timed("attention_prefill_quant", _d_attention_quant)
+def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+                            tile_item: torch.Tensor, tile_q0: torch.Tensor, item_tok_off: torch.Tensor, item_start: torch.Tensor,
+                            item_len: torch.Tensor, block_table: torch.Tensor, num_q_heads: int, scale: float, *, tile_rows: int = 64,
+                            max_keys: int = 0, num_splits: int = 0, out: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_prefill`` over the 8-bit cache: tiles of ``tile_rows`` consecutive query rows of prompt portions.  Tile i covers rows
+    [tile_q0[i], tile_q0[i]+tile_rows) of item tile_item[i] (-1: none); row r of an item sits at batch row item_tok_off[item]+r and at position
+    item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
+    ``attention_rows_quant``."""
+    hd, nt = k_cache.shape[-1], tile_item.shape[0]
+    _need(tile_item, "tile_item", torch.int32, (nt,))
+    _need(tile_q0, "tile_q0", torch.int32, (nt,))
+    for name, v in (("item_tok_off", item_tok_off), ("item_start", item_start), ("item_len", item_len)):
+        _need(v, name, torch.int32, (block_table.shape[0],))
+    if tile_rows < 1 or tile_rows > 65536:
+        raise KernelError(f"tiles of {tile_rows} rows")
+    out = _tile_out(q, out, num_q_heads * hd)
+    if nt == 0 or q.shape[0] == 0:
+        return out
+    if num_splits <= 0:
+        group = max(1, num_q_heads // k_cache.shape[1])
+        num_splits = tile_splits(nt * k_cache.shape[1] * max(1, tile_rows * group // 64), _key_bound(max_keys, block_table, k_cache.shape[2]),
+                                 _compute_units(q.device.index))
+    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, q.shape[0], int(num_splits), 0, out, workspace,
+                           tile_item=tile_item, tile_q0=tile_q0, item_tok_off=item_tok_off, item_start=item_start, item_len=item_len,
+                           num_tiles=nt, tile_rows=int(tile_rows))
+
+
+def _d_attention_shared(q, k_cache, v_cache, *a, **kw):
+    return {"rows": q.shape[0], "heads": q.shape[1] // k_cache.shape[3], "kv_heads": k_cache.shape[1], "head_dim": k_cache.shape[3],
+            "elem": k_cache.element_size()}
+
+
+@_timed("attention_shared", _d_attention_shared)
+def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, token_item: torch.Tensor, positions: torch.Tensor,
+                     block_table: torch.Tensor, num_q_heads: int, scale: float, row_start: torch.Tensor, shared_rows: torch.Tensor,
+                     group_off: torch.Tensor, *, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None,
+                     max_shared: int = 0, max_own: int = 0, shared_splits: int = 0, own_splits: int = 0,
+                     out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_rows`` for a batch whose requests begin with the same tokens, whose keys and values are read once for all of them.
+
+    Group i are the batch rows shared_rows[group_off[i] .. group_off[i+1]) (int32, a row in one group at most); row t of it reads the keys [0, row_start[t]), up to its
+    position, from the pages that the block table of the group's first row with a request names, and [row_start[t], position] through its own.
+    Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own; a row with
+    ``row_start`` > 0 has to be in a group.  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
+    All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
+    row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
+    ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 1)."""
+    T, hd = q.shape[0], k_cache.shape[-1]
+    if (k_exp is None) != (v_exp is None):
+        raise KernelError("an 8-bit cache has exponents of keys and of values")
+    for name, v in (("token_item", token_item), ("positions", positions), ("row_start", row_start)):
+        _need(v, name, torch.int32, (T,))
+    _need(shared_rows, "shared_rows", torch.int32, (shared_rows.shape[0],))
+    _need(group_off, "group_off", torch.int32, (group_off.shape[0],))
+    groups, n = group_off.shape[0] - 1, shared_rows.shape[0]
+    if groups < 1 or n < 1:
+        raise KernelError("attention_shared needs a group of rows (attention_rows and attention_rows_quant serve a batch without one)")
+    out = _tile_out(q, out, num_q_heads * hd)
+    if T == 0:
+        return out
+    nkv, units = k_cache.shape[1], _compute_units(q.device.index)
+    group = max(1, num_q_heads // nkv)
+    if shared_splits <= 0:
+        tiles = max(groups, n * group // 64)
+        shared_splits = tile_splits(tiles * nkv, _key_bound(max_shared, block_table, k_cache.shape[2]), units)
+    if own_splits <= 0:
+        own_splits = tile_splits(T * nkv, _key_bound(max_own, block_table, k_cache.shape[2]), units)
+    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, T, int(own_splits), int(shared_splits), out, workspace,
+                           token_item=token_item, positions=positions, row_start=row_start, shared_rows=shared_rows, group_off=group_off,
+                           num_entries=T, num_shared=n, num_groups=groups)
+
+
 # ---------------------------------------------------------------------- sampling
 def _d_sample(logits, **kw):
     return {"rows": logits.shape[0], "width": logits.shape[1], "bytes": logits.numel() * 4}
@@ -809,6 +1087,45 @@ def sample(logits: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
     _need(out, "out", torch.int32, (R,))
     _check(_lib().st_sample(_ptr(out), _ptr(logits), R, V, _ptr(temperature), _ptr(seeds), _ptr(draws),
                             _stream()))
+    return out
+
+
+def _d_sample_filtered(logits, *a, **kw):
+    return {"rows": logits.shape[0], "width": logits.shape[1], "bytes": logits.numel() * 4}
+
+
+@_timed("sample_filtered", _d_sample_filtered)
+def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor, *,
+                    top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                    min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Token ids [R] (int32) from float logits [R, V] (rows of any stride) and a random number of [0, 1) a row.
+
+    Weights are exp((logit - largest) / temperature).  In the order of values, the lower index first among equals, the
+    first ``top_k`` stay (int32 [R]; <= 0: all), of those the fewest whose weights make up ``top_p`` of theirs (float [R]; >= 1: all),
+    of those the ones with at least ``min_p`` of the largest weight (float [R]; <= 0: all).  The token is the first index,
+    upwards, at which the sum of the weights that stayed exceeds ``uniforms`` times all of it.  Rows with temperature <= 0 take the largest
+    logit, lowest index among equals.  Weights are whole numbers of 2^-44 of the largest, so results do not depend on any order
+    of summation.  A NaN logit is never chosen unless the row has nothing else.  Up to 2^18 logits a row."""
+    R, V = logits.shape
+    _need(logits, "logits", torch.float32, (R, V), contiguous=False)
+    if V < 1 or V > 1 << 18:
+        raise KernelError(f"sample_filtered takes 1 to {1 << 18} logits a row, not {V}")
+    if logits.stride(1) != 1 and V > 1:
+        raise KernelError("logits: rows must be dense")
+    _need(uniforms, "uniforms", torch.float32, (R,))
+    _need(temperature, "temperature", torch.float32, (R,))
+    for name, t, dt in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None:
+            _need(t, name, dt, (R,))
+    if out is None:
+        out = torch.empty((R,), dtype=torch.int32, device=logits.device)
+    _need(out, "out", torch.int32, (R,))
+    _on_one_device(logits, uniforms, temperature, top_k, top_p, min_p, out)
+    stride = max(logits.stride(0), V) if R > 1 else V
+    if R > 1 and logits.stride(0) < V:
+        raise KernelError("logits: rows overlap")
+    _check(_lib().st_sample_filtered(_ptr(out), _ptr(logits), stride, R, V, _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                     _ptr(min_p), _stream()))
     return out
 
 
