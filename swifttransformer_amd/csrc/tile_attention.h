@@ -19,6 +19,8 @@
 #include "api.h"
 #include "small_float.h"
 
+#include <type_traits>
+
 namespace st {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -107,6 +109,9 @@ __device__ inline void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// subtiles of 16 dims that the waves' results are joined by at a time: so many that each thread has a quad of a row's dims (16 rows: 4 subtiles)
+template <int RT> constexpr int turn_subtiles() { return RT == 1 ? 4 : RT == 2 ? 2 : 1; }
+
 constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
 
 // What a workgroup works on: rows [first, first + count) of the flat list (token j, query head) = (f / group, f % group).
@@ -116,27 +121,39 @@ struct TileWork {
     int lo;                // first key
     int kind;              // 0 one token, 1 consecutive rows of an item, 2 a list of rows over a prefix
     int base;              // the token; the item's first batch row; the list's first place
-    int start;             // kind 1: position of the item's first row
+    int start;             // kinds 0 and 1: position of the first row's token
     int slot, splits, split;
 };
 
 // flat row j's token and how many keys it sees; -1 where there is none
 __device__ inline int row_token(const StTileAttention& p, const TileWork& w, int j, int& sees) {
-    int t = w.base + j;
-    if (w.kind == 2) t = p.shared_rows[t];
+    const int t = w.kind == 2 ? p.shared_rows[w.base + j] : w.base + j;
     sees = 0;
     if (t < 0 || t >= p.num_rows) return -1;
-    if (w.kind == 1) {
-        sees = w.start + j + 1;
+    if (w.kind == 2) {
+        const int item = p.token_item[t], pos = p.positions[t], start = p.row_start[t];
+        if ((uint32_t)item < (uint32_t)p.num_items) sees = min(pos + 1, start);      // (else a padding row)
     } else {
-        sees = p.positions[t] + 1;
-        if (w.kind == 2) sees = min(sees, p.row_start[t]);
-        if ((uint32_t)p.token_item[t] >= (uint32_t)p.num_items) sees = 0;      // (no request: a padding row)
+        sees = w.start + j + 1;
     }
     return t;
 }
 
-template <typename TQ, typename TC, int HDP, int RT>
+// the largest (or least) over a row of 16 lanes, to all of them
+template <bool MAX>
+__device__ inline int row16(int x) {
+    const auto turn = [&](auto ctrl) {
+        const int y = __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, false);
+        x = MAX ? max(x, y) : min(x, y);
+    };
+    turn(std::integral_constant<int, 0x128>());
+    turn(std::integral_constant<int, 0x124>());
+    turn(std::integral_constant<int, 0x122>());
+    turn(std::integral_constant<int, 0x121>());
+    return x;
+}
+
+template <typename TQ, typename TC, int HDP, int RT, bool WHOLE>
 __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, int kvh, char* lds) {
     constexpr int DT = 2 * HDP, R = 16 * RT;
     constexpr bool QUANT = sizeof(TC) == 1;
@@ -148,8 +165,9 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     const int G = p.heads / p.kv_heads, hd = p.head_dim, ps = p.page_size;
     float* s_m = reinterpret_cast<float*>(lds);             // [4][R] the waves' maxima
     float* s_l = s_m + 4 * R;                               // [4][R] and normalisers
-    float* s_unit = s_l + 4 * R + wave * 64;                // a wave's keys' and values' powers of two
-    char* s_big = reinterpret_cast<char*>(s_l + 4 * R + (QUANT ? 256 : 0));
+    int* s_t = reinterpret_cast<int*>(s_l + 4 * R);         // [R] the rows' tokens
+    float* s_unit = s_l + 5 * R + wave * 64;                // a wave's keys' and values' powers of two
+    char* s_big = reinterpret_cast<char*>(s_l + 5 * R + (QUANT ? 256 : 0));
     char* s_v = s_big + wave * VB;                          // [4][32 values], at the end the waves' sums
 
     // ---- query rows
@@ -174,78 +192,107 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             if (t < 0 || d >= hd) clear(r);
             to_op(r, qf[rt][s]);
         }
+        if (wave == 0 && g == 0) s_t[16 * rt + r16] = t;
         most = max(most, sees);
         lim[rt] = t < 0 ? 0x7fffffff : sees;                // (a row that is none takes whatever comes)
         least = min(least, lim[rt]);
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        most = max(most, __shfl_xor(most, o, 64));
-        least = min(least, __shfl_xor(least, o, 64));
-    }
-    most = __builtin_amdgcn_readfirstlane(most);
-    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(row16<true>(most));
+    least = __builtin_amdgcn_readfirstlane(row16<false>(least));
 
-    // ---- keys of this workgroup: [kb, ke)
-    const int len = max(most - w.lo, 0);
+    // ---- keys of this workgroup: [kb0, ke), from a multiple of 16 on (keys before w.lo are masked)
+    const int lo = w.lo & ~15, len = max(most - lo, 0);
     const int blocks = (len + 31) >> 5, share = (blocks + w.splits - 1) / w.splits * 32;
-    const int64_t from = (int64_t)w.lo + (int64_t)w.split * share;
-    const int kb0 = (int)min(from, (int64_t)most), ke = (int)min(from + share, (int64_t)most);
+    const int64_t from = (int64_t)lo + (int64_t)w.split * share;
+    const int kb0 = w.lo < most ? (int)min(from, (int64_t)most) : 0, ke = w.lo < most ? (int)min(from + share, (int64_t)most) : 0;
 
+    // Pages.  WHOLE: 16 divides the page size, so 16 keys lie in one page; its number comes by a scalar load, and what a lane adds to its
+    // address never changes (but past the last key, which stands for those behind it).  Else every lane looks up its own keys.  Page
+    // numbers are asked for a block ahead of the entries, and before them: loads come back in order, and what is behind the entries of a
+    // block could not be used before all of them are there.  Nothing touches an entry between its load and its use, which would be a wait.
     const bool shifts = (ps & (ps - 1)) == 0;
     const int page_bits = 31 - __builtin_clz(ps);
     const int* bt = p.block_table + (int64_t)w.item * p.max_pages;
-    struct Place { int page, row; };
-    const auto look_up = [&](int key) {                     // (a key past the last one stands for that)
-        key = min(key, ke - 1);
-        const int pi = shifts ? key >> page_bits : key / ps;
-        return Place{bt[pi], key - pi * ps};
+    typedef const __attribute__((address_space(4))) int* scalar_ints;
+    const auto page_of = [&](int key) { return shifts ? key >> page_bits : key / ps; };
+    struct Places {
+        int page[2], row[2];                                // WHOLE: of 16 keys each, the page and the row of the first
+        int kp[2], kr[2], vp[2], vr[2], ep, er;             // else of each lane's keys
     };
-    Raw8<TC> kr[2][HDP];
-    uint4 vr[2][NV];
-    float unit = 0.f;
-    struct Places { Place k[2], v[2], e; };
     const auto look_up_block = [&](int kb) {
         Places q;
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            q.k[u] = look_up(kb + 16 * u + r16);
-            q.v[u] = look_up(kb + 16 * u + (lane >> 2));
+            for (int u = 0; u < 2; ++u) {
+                const int key = __builtin_amdgcn_readfirstlane(min(kb + 16 * u, ke - 1)), pi = page_of(key);
+                q.page[u] = *(scalar_ints)(uintptr_t)(bt + pi);
+                q.row[u] = key - pi * ps;
+            }
+        } else {
+            const auto look_up = [&](int key, int& page, int& row) {
+                key = min(key, ke - 1);
+                const int pi = page_of(key);
+                page = bt[pi];
+                row = key - pi * ps;
+            };
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                look_up(kb + 16 * u + r16, q.kp[u], q.kr[u]);
+                look_up(kb + 16 * u + (lane >> 2), q.vp[u], q.vr[u]);
+            }
+            if (QUANT) look_up(kb + (lane & 31), q.ep, q.er);
         }
-        if (QUANT) q.e = look_up(kb + (lane & 31));
         return q;
     };
-    uint64_t bad[2];                                        // keys whose page is none of the pool's
-    const auto issue = [&](const Places& q) {
+    struct Block {
+        Raw8<TC> kr[2][HDP];
+        uint4 vr[2][NV];
+        uint32_t field;                                     // exponent of a key's or (upper lanes) value's power of two
+        uint32_t bad;                                       // keys whose page is none of the pool's
+    };
+    const int head_off = kvh * ps * hd;
+    const bool outside = hd < 32 * HDP;                     // some lanes hold dims that the head does not have
+    uint32_t k_dims[HDP], v_bytes[NV];                      // what a lane adds for its dims (those outside: the row's start)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bool none = (uint32_t)q.k[u].page >= (uint32_t)p.num_pages;
-            bad[u] = __ballot(none);
-            const TC* at = (const TC*)p.k_cache + (uint64_t)(none ? 0u : (uint32_t)q.k[u].page) * (uint64_t)p.page_stride + (kvh * ps + q.k[u].row) * hd;
+    for (int s = 0; s < HDP; ++s) k_dims[s] = 32 * s + 8 * g < hd ? 32 * s + 8 * g : 0;
 #pragma unroll
-            for (int s = 0; s < HDP; ++s) {
-                const int d = 32 * s + 8 * g;
-                kr[u][s] = raw8(at + (d < hd ? d : 0));
-                if (d >= hd) clear(kr[u][s]);
+    for (int c = 0; c < NV; ++c) v_bytes[c] = 16 * (4 * c + (lane & 3)) < hd * ES ? 16 * (4 * c + (lane & 3)) : 0;
+    const auto load_keys = [&](Block& b, int u, const TC* at, uint32_t off) {
+#pragma unroll
+        for (int s = 0; s < HDP; ++s) b.kr[u][s] = raw8(at + (off + k_dims[s]));
+    };
+    const auto load_values = [&](Block& b, int u, const TC* at, uint32_t off) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) b.vr[u][c] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(at) + (off * ES + v_bytes[c]));
+    };
+    const auto issue = [&](Block& b, const Places& q, int kb) {
+        b.bad = 0;
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bool none = (uint32_t)q.page[u] >= (uint32_t)p.num_pages;
+                const int64_t at = (int64_t)(none ? 0 : q.page[u]) * p.page_stride + head_off + q.row[u] * hd;
+                const int left = max(ke - 1 - (kb + 16 * u), 0);         // rows behind the first that exist
+                load_keys(b, u, (const TC*)p.k_cache + at, (uint32_t)(min(r16, left) * hd));
+                load_values(b, u, (const TC*)p.v_cache + at, (uint32_t)(min(lane >> 2, left) * hd));
+                if (none) b.bad |= 0xffffu << (16 * u);
             }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const bool none = (uint32_t)q.v[u].page >= (uint32_t)p.num_pages;
-            const char* at = (const char*)((const TC*)p.v_cache + (uint64_t)(none ? 0u : (uint32_t)q.v[u].page) * (uint64_t)p.page_stride +
-                                           (kvh * ps + q.v[u].row) * hd);
-#pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const int b = 16 * (4 * c + (lane & 3));
-                vr[u][c] = *reinterpret_cast<const uint4*>(at + (b < hd * ES ? b : 0));
-                if (none) vr[u][c] = make_uint4(0, 0, 0, 0);
+            if (QUANT) {
+                const bool second = (lane >> 4) & 1;
+                const uint32_t page = second ? q.page[1] : q.page[0];
+                const int row = second ? q.row[1] : q.row[0], left = max(ke - 1 - (kb + (second ? 16 : 0)), 0);
+                b.field = (lane < 32 ? p.k_exp : p.v_exp)[(uint64_t)(page < (uint32_t)p.num_pages ? page : 0u) * (uint64_t)p.exp_stride + kvh * ps + row + min(r16, left)];
             }
-        }
-        if (QUANT) {
-            const bool none = (uint32_t)q.e.page >= (uint32_t)p.num_pages;
-            const uint8_t* e = lane < 32 ? p.k_exp : p.v_exp;
-            const uint32_t field = e[(uint64_t)(none ? 0u : (uint32_t)q.e.page) * (uint64_t)p.exp_stride + kvh * ps + q.e.row];
-            unit = none ? 1.f : __uint_as_float(field << 23);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bool none = (uint32_t)q.kp[u] >= (uint32_t)p.num_pages, vnone = (uint32_t)q.vp[u] >= (uint32_t)p.num_pages;
+                b.bad |= ((uint32_t)__ballot(none) & 0xffffu) << (16 * u);
+                load_keys(b, u, (const TC*)p.k_cache + (uint64_t)(none ? 0u : (uint32_t)q.kp[u]) * (uint64_t)p.page_stride + head_off, (uint32_t)(q.kr[u] * hd));
+                load_values(b, u, (const TC*)p.v_cache + (uint64_t)(vnone ? 0u : (uint32_t)q.vp[u]) * (uint64_t)p.page_stride + head_off, (uint32_t)(q.vr[u] * hd));
+            }
+            if (QUANT)
+                b.field = (lane < 32 ? p.k_exp : p.v_exp)[(uint64_t)((uint32_t)q.ep < (uint32_t)p.num_pages ? (uint32_t)q.ep : 0u) * (uint64_t)p.exp_stride + kvh * ps + q.er];
         }
     };
 
@@ -260,14 +307,19 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     }
     const float sl = p.scale * 1.44269504088896340736f;     // scores in units of log2
 
-    int kb = kb0 + 32 * wave;
-    Places next;
-    if (kb < ke) {
-        next = look_up_block(kb);
-        issue(next);
-        next = look_up_block(kb + 128);
-    }
-    for (; kb < ke; kb += 128) {
+    // a block in registers -> maximum, normaliser and sums; `then` is called once its registers are free
+    // (Without branches from the scores' products to the sums: what the compiler knows of a product's result and of loads under way ends at one.)
+    const auto consume = [&](Block& b, int kb, auto then) {
+        const uint32_t none = b.bad;
+        if (none != 0) {                                    // (their values are not to be multiplied, not even by nothing)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if ((none >> (16 * u + (lane >> 2))) & 1)
+#pragma unroll
+                    for (int c = 0; c < NV; ++c) b.vr[u][c] = make_uint4(0, 0, 0, 0);
+            if ((none >> (lane & 31)) & 1) b.field = 127;
+        }
+        const bool whole = kb >= w.lo && kb + 32 <= min(ke, least) && none == 0;
         floatx4 sc[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -276,7 +328,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 Op8<TQ> a;
-                to_op(kr[u][s], a);
+                if (outside && 32 * s + 8 * g >= hd) clear(b.kr[u][s]);
+                to_op(b.kr[u][s], a);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
             }
@@ -285,15 +338,12 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < NV; ++c) {
-                const int b = 16 * (4 * c + (lane & 3));
-                if (b < hd * ES) *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP>::kPitch + b) = vr[u][c];
+                const int at = 16 * (4 * c + (lane & 3));
+                if (64 * NV <= 32 * HDP * ES || at < 32 * HDP * ES)
+                    *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP>::kPitch + at) = b.vr[u][c];
             }
-        if (QUANT) s_unit[lane] = unit;
-        const uint64_t bad0 = bad[0], bad1 = bad[1];
-        if (kb + 128 < ke) {
-            issue(next);
-            next = look_up_block(kb + 256);
-        }
+        if (QUANT) s_unit[lane] = __uint_as_float(b.field << 23);
+        then();                                             // (the block's registers are free)
         wave_fence();
         floatx4 ku[2], vu[2];
         if (QUANT) {
@@ -303,22 +353,29 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 vu[u] = *reinterpret_cast<const floatx4*>(s_unit + 32 + 16 * u + 4 * g);
             }
         }
-        const bool whole = kb + 32 <= min(ke, least) && (bad0 | bad1) == 0;
+        float x[RT][8];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[rt][i] = sc[rt][i >> 2][i & 3] * sl;
+                if (QUANT) x[rt][i] *= ku[i >> 2][i & 3];
+            }
+        if (!whole) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int in = 16 * (i >> 2) + 4 * g + (i & 3), key = kb + in;
+                    if ((key >= min(ke, lim[rt])) | (key < w.lo) | ((none >> in) & 1)) x[rt][i] = -INFINITY;
+                }
+        }
         Op8<TQ> pf[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float x[8], top = -INFINITY;
+            float top = max_raw(x[rt][0], x[rt][1]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int u = i >> 2, r = i & 3;
-                x[i] = sc[rt][u][r] * sl;
-                if (QUANT) x[i] *= ku[u][r];
-                if (!whole) {
-                    const int key = kb + 16 * u + 4 * g + r;
-                    if (key >= min(ke, lim[rt]) || (((u ? bad1 : bad0) >> (4 * g + r)) & 1)) x[i] = -INFINITY;
-                }
-                top = max_raw(top, x[i]);
-            }
+            for (int i = 2; i < 8; i += 2) top = max3_raw(top, x[rt][i], x[rt][i + 1]);
             top = rows4_max(top);
             const float mn = max_raw(m[rt], top);
             if (__any(mn > m[rt])) {
@@ -330,20 +387,47 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(x[i] - mn);
-                l[rt] += x[i];
-                if (QUANT) x[i] *= vu[i >> 2][i & 3];
+                x[rt][i] = __builtin_amdgcn_exp2f(x[rt][i] - mn);
+                l[rt] += x[rt][i];
+                if (QUANT) x[rt][i] *= vu[i >> 2][i & 3];
             }
-            weights_to_op(x, pf[rt]);
+            weights_to_op(x[rt], pf[rt]);
         }
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            if (16 * dt < hd) {
-                Op8<TQ> v;
-                value_op<HDP>(s_v, dt, g, r16, TC{}, v);
+        for (int dt = 0; dt < DT; ++dt) {                   // (dims that the head does not have: never stored)
+            Op8<TQ> v;
+            value_op<HDP>(s_v, dt, g, r16, TC{}, v);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt], acc[rt][dt]);
+            for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt], acc[rt][dt]);
+        }
+    };
+    int kb = kb0 + 32 * wave;
+    Places next;
+    const auto ahead = [&](Block& b, int at) {              // asks for the block at `at`, whose pages are known, and for the pages of the one behind
+        const Places now = next;                            // (whether or not there is one: what is asked for twice is the last key)
+        next = look_up_block(at + 128);
+        issue(b, now, at);
+    };
+    Block one;
+    if (kb < ke) {
+        next = look_up_block(kb);
+        ahead(one, kb);
+        if constexpr (RT == 1) {                            // few rows: two blocks, one on its way while the other is used
+            Block two;
+            for (;;) {
+                ahead(two, kb + 128);
+                __builtin_amdgcn_sched_barrier(0);
+                consume(one, kb, [] {});
+                __builtin_amdgcn_sched_barrier(0);
+                if ((kb += 128) >= ke) break;
+                ahead(one, kb + 128);
+                __builtin_amdgcn_sched_barrier(0);
+                consume(two, kb, [] {});
+                __builtin_amdgcn_sched_barrier(0);
+                if ((kb += 128) >= ke) break;
             }
+        } else {
+            for (; kb < ke; kb += 128) consume(one, kb, [&] { ahead(one, kb + 128); });
         }
     }
 
@@ -367,41 +451,41 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= own;
     }
     // a thread's row and four of its dims, in turns over the subtiles of the head
-    constexpr int JP = 20;                                  // floats between rows of a subtile in LDS
+    constexpr int DC = turn_subtiles<RT>(), JP = 16 * DC + 4;       // subtiles a turn, floats between its rows in LDS
     float* s_o = reinterpret_cast<float*>(s_big);           // [4][R][JP]
-    const int row = tid >> 2, quad = tid & 3;               // (R <= 64)
-    int t = -1, sees = 0, head = 0;
+    constexpr int TPR = 256 / R;                            // threads a row, a quad of dims each
+    const int row = tid / TPR, quad = tid % TPR;
+    const int f = w.first + row, t = s_t[row], head = kvh * G + f - f / G * G;
     float top = kFloor, sum = 0.f;
-    if (row < R) {
-        const int f = w.first + row;
-        if (f < w.count) {
-            const int j = f / G;
-            head = kvh * G + f - j * G;
-            t = row_token(p, w, j, sees);
-        }
-        for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + row]);
-        for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * __builtin_amdgcn_exp2f(s_m[v * R + row] - top);
-    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + row]);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * __builtin_amdgcn_exp2f(s_m[v * R + row] - top);
     // (a sum that is no number belongs to the result)
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t out_row = (int64_t)(w.slot >= 0 ? w.slot : t) * p.heads + head;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-        if (16 * dt >= hd) break;
+    for (int d0 = 0; d0 < DT; d0 += DC) {
+        if (16 * d0 >= hd) break;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) *reinterpret_cast<floatx4*>(s_o + (wave * R + 16 * rt + r16) * JP + 4 * g) = acc[rt][dt];
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int c = 0; c < DC; ++c)
+                if (16 * rt + r16 + w.first < w.count && 16 * (d0 + c) < hd)
+                    *reinterpret_cast<floatx4*>(s_o + (wave * R + 16 * rt + r16) * JP + 16 * c + 4 * g) = acc[rt][d0 + c];
         __syncthreads();
-        if (t >= 0) {
+        const int d = 16 * d0 + 4 * quad;
+        if (t >= 0 && d < hd) {
             floatx4 o = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; ++v) o += *reinterpret_cast<const floatx4*>(s_o + (v * R + row) * JP + 4 * quad);
             const float res[4] = {o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse};
             if (p.slots == 1)
-                Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + 16 * dt + 4 * quad, res);
+                Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + d, res);
             else
-                Elem<float>::store4(p.part_o + (out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split) * hd + 16 * dt + 4 * quad, res);
+                Elem<float>::store4(p.part_o + (out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split) * hd + d, res);
         }
-        __syncthreads();
+        if (d0 + DC < DT) __syncthreads();
     }
     if (t >= 0 && p.slots > 1 && quad == 0)
         p.part_lse[out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split] = sum == 0.f ? -INFINITY : top + log2f(sum);
@@ -410,13 +494,14 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 // LDS of a workgroup
 template <typename TQ, typename TC, int HDP, int RT>
 constexpr int tile_lds() {
-    return (2 * 4 * 16 * RT + (sizeof(TC) == 1 ? 256 : 0)) * 4 +
-           (4 * Values<TC, HDP>::kBytes > 4 * 16 * RT * 20 * 4 ? 4 * Values<TC, HDP>::kBytes : 4 * 16 * RT * 20 * 4);
+    constexpr int kTurn = 4 * 16 * RT * (16 * turn_subtiles<RT>() + 4) * 4;
+    return (9 * 16 * RT + (sizeof(TC) == 1 ? 256 : 0)) * 4 +
+           (4 * Values<TC, HDP>::kBytes > kTurn ? 4 * Values<TC, HDP>::kBytes : kTurn);
 }
 
 // Workgroups: key head fastest (a head's workgroups share its keys and, dealt out in turn, an XCD's L2), then splits, then
 // entries: shared prefixes first (kind 2, RTS subtiles of rows), then single tokens or tiles (RT).
-template <typename TQ, typename TC, int HDP, int RT, int RTS>
+template <typename TQ, typename TC, int HDP, int RT, int RTS, bool WHOLE>
 __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttention p) {
     extern __shared__ uint4 dyn[];
     char* lds = reinterpret_cast<char*>(dyn);
@@ -426,7 +511,7 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
     TileWork w;
     w.start = w.lo = 0;
     w.slot = -1;
-    if (RTS > 0) {
+    if constexpr (RTS > 0) {
         if (y < p.shared_entries * p.shared_splits) {
             int e = y / p.shared_splits;
             w.split = y - e * p.shared_splits;
@@ -466,7 +551,7 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
             const uint64_t there = __ballot((uint32_t)item < (uint32_t)p.num_items);
             if (!there) w.lo = 0x7fffffff;                 // none: no key is seen
             w.item = there ? __builtin_amdgcn_readfirstlane(__shfl(item, __ffsll((unsigned long long)there) - 1, 64)) : 0;
-            tile_work<TQ, TC, HDP, (RTS > 0 ? RTS : 1)>(p, w, kvh, lds);
+            tile_work<TQ, TC, HDP, (RTS > 0 ? RTS : 1), WHOLE>(p, w, kvh, lds);
             return;
         }
         y -= p.shared_entries * p.shared_splits;
@@ -500,11 +585,16 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
         w.base = t;
         w.first = (entry - ri * chunks) * R;
         w.count = G;
-        w.item = p.token_item[t];
-        if ((uint32_t)w.item >= (uint32_t)p.num_items) w.item = 0;         // (a padding row sees no key)
-        if (p.row_start) w.lo = max(p.row_start[t], 0);
+        // (asked for together, by the scalar unit)
+        w.item = __builtin_amdgcn_readfirstlane(p.token_item[t]);
+        w.start = __builtin_amdgcn_readfirstlane(p.positions[t]);
+        if (RTS > 0) w.lo = max(__builtin_amdgcn_readfirstlane(p.row_start[t]), 0);
+        if ((uint32_t)w.item >= (uint32_t)p.num_items) {                   // a padding row sees no key
+            w.item = 0;
+            w.start = -1;
+        }
     }
-    tile_work<TQ, TC, HDP, RT>(p, w, kvh, lds);
+    tile_work<TQ, TC, HDP, RT, WHOLE>(p, w, kvh, lds);
 }
 
 // out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s, w_s = 2^(lse_s - max lse): one wave a row and head
@@ -543,7 +633,7 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p
 
 // The instances of a query type: for heads of up to 64, 96, 128 and 256 dims; rows in subtiles of 16: one for single tokens (a
 // group's heads), MAX for tiles and long lists of rows.
-template <typename TQ, typename TC, int HDP, int RT, int RTS>
+template <typename TQ, typename TC, int HDP, int RT, int RTS, bool WHOLE>
 int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     constexpr int lds1 = tile_lds<TQ, TC, HDP, RT>(), lds2 = RTS > 0 ? tile_lds<TQ, TC, HDP, (RTS > 0 ? RTS : 1)>() : 0;
     const int G = p.heads / p.kv_heads;
@@ -556,9 +646,9 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     if (groups == 0) return 0;
     constexpr int lds = lds1 > lds2 ? lds1 : lds2;
     if constexpr (lds > 64 * 1024)
-        ST_CHECK(hipFuncSetAttribute((const void*)tile_attention_kernel<TQ, TC, HDP, RT, RTS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
+        ST_CHECK(hipFuncSetAttribute((const void*)tile_attention_kernel<TQ, TC, HDP, RT, RTS, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
                  "attention: %d bytes of LDS refused", lds);
-    tile_attention_kernel<TQ, TC, HDP, RT, RTS><<<(unsigned)groups, 256, lds, stream>>>(q);
+    tile_attention_kernel<TQ, TC, HDP, RT, RTS, WHOLE><<<(unsigned)groups, 256, lds, stream>>>(q);
     ST_LAUNCH_CHECK("tile_attention");
     if (p.slots > 1) {
         const int64_t rows = p.num_tiles > 0 ? (int64_t)p.num_tiles * p.tile_rows : p.num_entries;
@@ -568,25 +658,34 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     return 0;
 }
 
-template <typename TQ, int HDP, int MAX>
+// (Pages that 16 does not divide go by subtiles of 16 rows only.)
+template <typename TQ, typename TC, int HDP, int MAX>
 int launch_tiles_of(const StTileAttention& p, hipStream_t stream) {
     const bool many = (int64_t)p.num_shared * (p.heads / p.kv_heads) > 16 * (int64_t)p.num_groups;
-    if (p.cache_dtype == 2) {
-        if (p.num_groups > 0) return many ? launch_tiles<TQ, e4m3_t, HDP, 1, MAX>(p, stream) : launch_tiles<TQ, e4m3_t, HDP, 1, 1>(p, stream);
-        return p.num_tiles > 0 ? launch_tiles<TQ, e4m3_t, HDP, MAX, 0>(p, stream) : launch_tiles<TQ, e4m3_t, HDP, 1, 0>(p, stream);
+    if (p.num_groups > 0) {
+        if (p.page_size % 16 != 0) return launch_tiles<TQ, TC, HDP, 1, 1, false>(p, stream);
+        return many ? launch_tiles<TQ, TC, HDP, 1, MAX, true>(p, stream) : launch_tiles<TQ, TC, HDP, 1, 1, true>(p, stream);
     }
-    return many ? launch_tiles<TQ, TQ, HDP, 1, MAX>(p, stream) : launch_tiles<TQ, TQ, HDP, 1, 1>(p, stream);
+    if constexpr (sizeof(TC) == 1) {
+        if (p.page_size % 16 != 0) return launch_tiles<TQ, TC, HDP, 1, 0, false>(p, stream);
+        return p.num_tiles > 0 ? launch_tiles<TQ, TC, HDP, MAX, 0, true>(p, stream) : launch_tiles<TQ, TC, HDP, 1, 0, true>(p, stream);
+    }
+    ST_CHECK(false, "attention: a cache of the queries' type goes by groups");
+    return 0;
 }
 
-template <typename TQ, int MAX>
+template <typename TQ, typename TC, int MAX>
 int launch_tiles_by_head(const StTileAttention& p, hipStream_t stream) {
-    if (p.head_dim <= 64) return launch_tiles_of<TQ, 2, MAX>(p, stream);
-    if (p.head_dim <= 96) return launch_tiles_of<TQ, 3, MAX>(p, stream);
-    if (p.head_dim <= 128) return launch_tiles_of<TQ, 4, MAX>(p, stream);
-    return launch_tiles_of<TQ, 8, MAX / 2>(p, stream);
+    if (p.head_dim <= 64) return launch_tiles_of<TQ, TC, 2, MAX>(p, stream);
+    if (p.head_dim <= 96) return launch_tiles_of<TQ, TC, 3, MAX>(p, stream);
+    if (p.head_dim <= 128) return launch_tiles_of<TQ, TC, 4, MAX>(p, stream);
+    return launch_tiles_of<TQ, TC, 8, MAX / 2>(p, stream);
 }
 
+// the sources that hold them: by the queries' type and the cache's
 int tile_attention_bf16(const StTileAttention& p, hipStream_t stream);
+int tile_attention_bf16_quant(const StTileAttention& p, hipStream_t stream);
 int tile_attention_f32(const StTileAttention& p, hipStream_t stream);
+int tile_attention_f32_quant(const StTileAttention& p, hipStream_t stream);
 
 }  // namespace st

@@ -1,8 +1,8 @@
-// The bfloat16 instances of csrc/tile_attention.h, and its C entry.
+// csrc/tile_attention.h for bfloat16 queries over a bfloat16 cache, and its C entry.
 #include "tile_attention.h"
 
 namespace st {
-int tile_attention_bf16(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<bf16_t, 4>(p, stream); }
+int tile_attention_bf16(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<bf16_t, bf16_t, 4>(p, stream); }
 }  // namespace st
 
 using namespace st;
@@ -31,5 +31,6 @@ extern "C" int st_tile_attention(const StTileAttention* args, hipStream_t stream
     ST_CHECK(((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache) |
                reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.part_o)) & 15) == 0 && p.q_stride * (p.dtype == kF32 ? 4 : 2) % 16 == 0,
              "attention: queries, their rows, caches and results must be 16-byte aligned");
+    if (p.cache_dtype == 2) return p.dtype == kBF16 ? tile_attention_bf16_quant(p, stream) : tile_attention_f32_quant(p, stream);
     return p.dtype == kBF16 ? tile_attention_bf16(p, stream) : tile_attention_f32(p, stream);
 }

@@ -39,7 +39,11 @@ HIPCC_FLAGS = [
 FILE_FLAGS = {"attention_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_prefill_dma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_prefill_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-              "latent_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+              "latent_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "tile_attention_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "tile_attention_bf16_quant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "tile_attention_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "tile_attention_f32_quant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # Files whose loads stay where the sources ask for them.  Many kernels clamp a load's address and clear afterwards what should not be there, so
 # that a batch of loads is on its way together; the optimiser may move such a load to the one place that uses it, behind the lane's condition,
 # where each waits for its own trip to memory.  Left in place they hold registers longer, so a file is here only where both ways were timed
