@@ -3,7 +3,7 @@
 //
 // A workgroup takes one key head, up to 16 * RT query rows and a share of the keys.  Query rows are (token, query head of the key head's
 // group) pairs: the heads of one token, of the tokens of a prompt's portion, or of all tokens whose requests begin with the same pages.
-// A key is then read once for all of them.  Its four waves take blocks of 32 keys in turn, each with a running maximum, normaliser and
+// A key is then read once for all of them.  Its four waves take blocks of 32 or 64 keys in turn, each with a running maximum, normaliser and
 // sum of its own (an online softmax in float), and meet in LDS at the end; several workgroups that share a row's keys leave
 // normalised sums and log-sum-exps, which a second kernel joins.
 //
@@ -74,22 +74,22 @@ __device__ inline void weights_to_op(const float* p, Op8<float>& o) {
     for (int i = 0; i < 8; ++i) o.v[i] = p[i];
 }
 
-// ---- a wave's block of 32 values in LDS: rows of kPitch bytes, and an operand of V^T from there: dim 16 * dt + l % 16, keys 4g .. 4g+3 and
+// ---- a wave's block of 16 NU values in LDS: rows of kPitch bytes, and an operand of V^T from 32 of them: dim 16 * dt + l % 16, keys 4g .. 4g+3 and
 // 16 + 4g .. 16 + 4g+3 (g = l / 16), the keys of the scores that the lane holds
-template <typename TC, int HDP> struct Values {
+template <typename TC, int HDP, int NU> struct Values {
     // (a pitch that keeps the rows of a transposing read on different banks)
     static constexpr int kPitch = 32 * HDP * (int)sizeof(TC) + (sizeof(TC) == 2 ? 32 : 16);
-    static constexpr int kBytes = 32 * kPitch;
+    static constexpr int kBytes = 16 * NU * kPitch;
 };
 template <int HDP> __device__ inline void value_op(const char* block, int dt, int g, int r16, bf16_t, Op8<bf16_t>& o) {
-    constexpr int P = Values<bf16_t, HDP>::kPitch;
+    constexpr int P = Values<bf16_t, HDP, 2>::kPitch;
     const char* at = block + (4 * g + (r16 >> 2)) * P + 32 * dt + 8 * (r16 & 3);
     const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(ST_LDS_PTR(short4v, at)));
     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(ST_LDS_PTR(short4v, at + 16 * P)));
     o.v = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
 }
 template <int HDP, typename TQ> __device__ inline void value_op(const char* block, int dt, int g, int r16, e4m3_t, Op8<TQ>& o) {
-    constexpr int P = Values<e4m3_t, HDP>::kPitch;
+    constexpr int P = Values<e4m3_t, HDP, 2>::kPitch;
     const int k = r16 >> 1;
     const char* at = block + ((k < 4 ? 4 * g + k : 12 + 4 * g + k)) * P + 16 * dt + 8 * (r16 & 1);
     Raw8<e4m3_t> r;
@@ -97,7 +97,7 @@ template <int HDP, typename TQ> __device__ inline void value_op(const char* bloc
     to_op(r, o);
 }
 template <int HDP> __device__ inline void value_op(const char* block, int dt, int g, int r16, float, Op8<float>& o) {
-    constexpr int P = Values<float, HDP>::kPitch;
+    constexpr int P = Values<float, HDP, 2>::kPitch;
     const char* at = block + 4 * g * P + 4 * (16 * dt + r16);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = *reinterpret_cast<const float*>(at + ((i & 3) + 16 * (i >> 2)) * P);
@@ -111,6 +111,14 @@ __device__ inline void wave_fence() {
 
 // subtiles of 16 dims that the waves' results are joined by at a time: so many that each thread has a quad of a row's dims (16 rows: 4 subtiles)
 template <int RT> constexpr int turn_subtiles() { return RT == 1 ? 4 : RT == 2 ? 2 : 1; }
+
+// Subtiles of 16 keys a block, and whether two blocks are held, one on its way while the other is used (where the registers do for that).
+template <typename TQ, typename TC, int HDP, int RT> struct Shape {
+    static constexpr int NU = RT == 1 && HDP == 2 ? 4 : 2;
+    static constexpr int NV = (2 * HDP * (int)sizeof(TC) + 3) / 4;             // 16-byte chunks of a value that a lane moves (four lanes a value)
+    static constexpr int kBlock = NU * (HDP * (int)sizeof(Raw8<TC>) / 4 + 4 * NV);
+    static constexpr bool kTwo = 2 * kBlock + RT * (HDP * (int)sizeof(Op8<TQ>) / 4 + 8 * HDP + 8 * NU) <= 416;
+};
 
 constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
 
@@ -158,17 +166,18 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     constexpr int DT = 2 * HDP, R = 16 * RT;
     constexpr bool QUANT = sizeof(TC) == 1;
     constexpr int ES = sizeof(TC);
-    constexpr int NV = (2 * HDP * ES + 3) / 4;             // 16-byte chunks of a value that a lane moves (four lanes a value)
-    constexpr int VB = Values<TC, HDP>::kBytes;
+    using S = Shape<TQ, TC, HDP, RT>;
+    constexpr int NU = S::NU, NV = S::NV, KEYS = 16 * NU, STEP = 4 * KEYS, NF = NU / 2;
+    constexpr int VB = Values<TC, HDP, NU>::kBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
     const int G = p.heads / p.kv_heads, hd = p.head_dim, ps = p.page_size;
     float* s_m = reinterpret_cast<float*>(lds);             // [4][R] the waves' maxima
     float* s_l = s_m + 4 * R;                               // [4][R] and normalisers
     int* s_t = reinterpret_cast<int*>(s_l + 4 * R);         // [R] the rows' tokens
-    float* s_unit = s_l + 5 * R + wave * 64;                // a wave's keys' and values' powers of two
-    char* s_big = reinterpret_cast<char*>(s_l + 5 * R + (QUANT ? 256 : 0));
-    char* s_v = s_big + wave * VB;                          // [4][32 values], at the end the waves' sums
+    float* s_unit = s_l + 5 * R + wave * 2 * KEYS;          // the powers of two of a wave's keys, then values
+    char* s_big = reinterpret_cast<char*>(s_l + 5 * R + (QUANT ? 8 * KEYS : 0));
+    char* s_v = s_big + wave * VB;                          // [4][KEYS values], at the end the waves' sums
 
     // ---- query rows
     Op8<TQ> qf[RT][HDP];
@@ -202,7 +211,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 
     // ---- keys of this workgroup: [kb0, ke), from a multiple of 16 on (keys before w.lo are masked)
     const int lo = w.lo & ~15, len = max(most - lo, 0);
-    const int blocks = (len + 31) >> 5, share = (blocks + w.splits - 1) / w.splits * 32;
+    const int blocks = (len + KEYS - 1) / KEYS, share = (blocks + w.splits - 1) / w.splits * KEYS;
     const int64_t from = (int64_t)lo + (int64_t)w.split * share;
     const int kb0 = w.lo < most ? (int)min(from, (int64_t)most) : 0, ke = w.lo < most ? (int)min(from + share, (int64_t)most) : 0;
 
@@ -216,14 +225,14 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     typedef const __attribute__((address_space(4))) int* scalar_ints;
     const auto page_of = [&](int key) { return shifts ? key >> page_bits : key / ps; };
     struct Places {
-        int page[2], row[2];                                // WHOLE: of 16 keys each, the page and the row of the first
-        int kp[2], kr[2], vp[2], vr[2], ep, er;             // else of each lane's keys
+        int page[NU], row[NU];                              // WHOLE: of 16 keys each, the page and the row of the first
+        int kp[NU], kr[NU], vp[NU], vr[NU], ep[NF], er[NF]; // else of each lane's keys
     };
     const auto look_up_block = [&](int kb) {
         Places q;
         if constexpr (WHOLE) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 const int key = __builtin_amdgcn_readfirstlane(min(kb + 16 * u, ke - 1)), pi = page_of(key);
                 q.page[u] = *(scalar_ints)(uintptr_t)(bt + pi);
                 q.row[u] = key - pi * ps;
@@ -236,19 +245,21 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 row = key - pi * ps;
             };
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 look_up(kb + 16 * u + r16, q.kp[u], q.kr[u]);
                 look_up(kb + 16 * u + (lane >> 2), q.vp[u], q.vr[u]);
             }
-            if (QUANT) look_up(kb + (lane & 31), q.ep, q.er);
+            if (QUANT)
+#pragma unroll
+                for (int f = 0; f < NF; ++f) look_up(kb + (64 * f + lane) % KEYS, q.ep[f], q.er[f]);
         }
         return q;
     };
     struct Block {
-        Raw8<TC> kr[2][HDP];
-        uint4 vr[2][NV];
-        uint32_t field;                                     // exponent of a key's or (upper lanes) value's power of two
-        uint32_t bad;                                       // keys whose page is none of the pool's
+        Raw8<TC> kr[NU][HDP];
+        uint4 vr[NU][NV];
+        uint32_t field[NF];                                 // exponents of the powers of two: lane l's number f is that of key 64 f + l, values behind keys
+        uint64_t bad;                                       // keys whose page is none of the pool's
     };
     const int head_off = kvh * ps * hd;
     const bool outside = hd < 32 * HDP;                     // some lanes hold dims that the head does not have
@@ -269,30 +280,46 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         b.bad = 0;
         if constexpr (WHOLE) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 const bool none = (uint32_t)q.page[u] >= (uint32_t)p.num_pages;
                 const int64_t at = (int64_t)(none ? 0 : q.page[u]) * p.page_stride + head_off + q.row[u] * hd;
                 const int left = max(ke - 1 - (kb + 16 * u), 0);         // rows behind the first that exist
                 load_keys(b, u, (const TC*)p.k_cache + at, (uint32_t)(min(r16, left) * hd));
                 load_values(b, u, (const TC*)p.v_cache + at, (uint32_t)(min(lane >> 2, left) * hd));
-                if (none) b.bad |= 0xffffu << (16 * u);
+                if (none) b.bad |= (uint64_t)0xffffu << (16 * u);
             }
             if (QUANT) {
-                const bool second = (lane >> 4) & 1;
-                const uint32_t page = second ? q.page[1] : q.page[0];
-                const int row = second ? q.row[1] : q.row[0], left = max(ke - 1 - (kb + (second ? 16 : 0)), 0);
-                b.field = (lane < 32 ? p.k_exp : p.v_exp)[(uint64_t)(page < (uint32_t)p.num_pages ? page : 0u) * (uint64_t)p.exp_stride + kvh * ps + row + min(r16, left)];
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    // (which of the block's 16 keys: a lane's sixteenth of a wave, keys or values)
+                    uint32_t page = q.page[0];
+                    int row = q.row[0], at = kb;
+#pragma unroll
+                    for (int u = 1; u < NU; ++u)
+                        if (((64 * f + lane) % KEYS) >> 4 == u) {
+                            page = q.page[u];
+                            row = q.row[u];
+                            at = kb + 16 * u;
+                        }
+                    const uint8_t* e = 64 * f + lane < KEYS ? p.k_exp : p.v_exp;
+                    b.field[f] = e[(uint64_t)(page < (uint32_t)p.num_pages ? page : 0u) * (uint64_t)p.exp_stride + kvh * ps + row + min(r16, max(ke - 1 - at, 0))];
+                }
             }
         } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 const bool none = (uint32_t)q.kp[u] >= (uint32_t)p.num_pages, vnone = (uint32_t)q.vp[u] >= (uint32_t)p.num_pages;
-                b.bad |= ((uint32_t)__ballot(none) & 0xffffu) << (16 * u);
+                b.bad |= (__ballot(none) & 0xffffu) << (16 * u);
                 load_keys(b, u, (const TC*)p.k_cache + (uint64_t)(none ? 0u : (uint32_t)q.kp[u]) * (uint64_t)p.page_stride + head_off, (uint32_t)(q.kr[u] * hd));
                 load_values(b, u, (const TC*)p.v_cache + (uint64_t)(vnone ? 0u : (uint32_t)q.vp[u]) * (uint64_t)p.page_stride + head_off, (uint32_t)(q.vr[u] * hd));
             }
-            if (QUANT)
-                b.field = (lane < 32 ? p.k_exp : p.v_exp)[(uint64_t)((uint32_t)q.ep < (uint32_t)p.num_pages ? (uint32_t)q.ep : 0u) * (uint64_t)p.exp_stride + kvh * ps + q.er];
+            if (QUANT) {
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const uint32_t page = (uint32_t)q.ep[f] < (uint32_t)p.num_pages ? (uint32_t)q.ep[f] : 0u;
+                    b.field[f] = (64 * f + lane < KEYS ? p.k_exp : p.v_exp)[(uint64_t)page * (uint64_t)p.exp_stride + kvh * ps + q.er[f]];
+                }
+            }
         }
     };
 
@@ -310,23 +337,27 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     // a block in registers -> maximum, normaliser and sums; `then` is called once its registers are free
     // (Without branches from the scores' products to the sums: what the compiler knows of a product's result and of loads under way ends at one.)
     const auto consume = [&](Block& b, int kb, auto then) {
-        const uint32_t none = b.bad;
+        const uint64_t none = b.bad;
         if (none != 0) {                                    // (their values are not to be multiplied, not even by nothing)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
                 if ((none >> (16 * u + (lane >> 2))) & 1)
 #pragma unroll
                     for (int c = 0; c < NV; ++c) b.vr[u][c] = make_uint4(0, 0, 0, 0);
-            if ((none >> (lane & 31)) & 1) b.field = 127;
-        }
-        const bool whole = kb >= w.lo && kb + 32 <= min(ke, least) && none == 0;
-        floatx4 sc[RT][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int f = 0; f < NF; ++f)
+                if ((none >> ((64 * f + lane) % KEYS)) & 1) b.field[f] = 127;
+        }
+        const bool whole = kb >= w.lo && kb + KEYS <= min(ke, least) && none == 0;
+        floatx4 sc[RT][NU];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) sc[rt][u] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < HDP; ++s)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 Op8<TQ> a;
                 if (outside && 32 * s + 8 * g >= hd) clear(b.kr[u][s]);
                 to_op(b.kr[u][s], a);
@@ -335,29 +366,31 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
         wave_fence();                                       // (the block before has been read)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
             for (int c = 0; c < NV; ++c) {
                 const int at = 16 * (4 * c + (lane & 3));
                 if (64 * NV <= 32 * HDP * ES || at < 32 * HDP * ES)
-                    *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP>::kPitch + at) = b.vr[u][c];
+                    *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP, NU>::kPitch + at) = b.vr[u][c];
             }
-        if (QUANT) s_unit[lane] = __uint_as_float(b.field << 23);
+        if (QUANT)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) s_unit[64 * f + lane] = __uint_as_float(b.field[f] << 23);
         then();                                             // (the block's registers are free)
         wave_fence();
-        floatx4 ku[2], vu[2];
+        floatx4 ku[NU], vu[NU];
         if (QUANT) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NU; ++u) {
                 ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
-                vu[u] = *reinterpret_cast<const floatx4*>(s_unit + 32 + 16 * u + 4 * g);
+                vu[u] = *reinterpret_cast<const floatx4*>(s_unit + KEYS + 16 * u + 4 * g);
             }
         }
-        float x[RT][8];
+        float x[RT][4 * NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * NU; ++i) {
                 x[rt][i] = sc[rt][i >> 2][i & 3] * sl;
                 if (QUANT) x[rt][i] *= ku[i >> 2][i & 3];
             }
@@ -365,17 +398,17 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 4 * NU; ++i) {
                     const int in = 16 * (i >> 2) + 4 * g + (i & 3), key = kb + in;
                     if ((key >= min(ke, lim[rt])) | (key < w.lo) | ((none >> in) & 1)) x[rt][i] = -INFINITY;
                 }
         }
-        Op8<TQ> pf[RT];
+        Op8<TQ> pf[RT][NF];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float top = max_raw(x[rt][0], x[rt][1]);
 #pragma unroll
-            for (int i = 2; i < 8; i += 2) top = max3_raw(top, x[rt][i], x[rt][i + 1]);
+            for (int i = 2; i < 4 * NU; i += 2) top = max3_raw(top, x[rt][i], x[rt][i + 1]);
             top = rows4_max(top);
             const float mn = max_raw(m[rt], top);
             if (__any(mn > m[rt])) {
@@ -386,48 +419,52 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 m[rt] = mn;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * NU; ++i) {
                 x[rt][i] = __builtin_amdgcn_exp2f(x[rt][i] - mn);
                 l[rt] += x[rt][i];
                 if (QUANT) x[rt][i] *= vu[i >> 2][i & 3];
             }
-            weights_to_op(x[rt], pf[rt]);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) weights_to_op(x[rt] + 8 * f, pf[rt][f]);
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {                   // (dims that the head does not have: never stored)
-            Op8<TQ> v;
-            value_op<HDP>(s_v, dt, g, r16, TC{}, v);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt], acc[rt][dt]);
+            for (int f = 0; f < NF; ++f) {
+                Op8<TQ> v;
+                value_op<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16, TC{}, v);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt][f], acc[rt][dt]);
+            }
         }
     };
-    int kb = kb0 + 32 * wave;
+    int kb = kb0 + KEYS * wave;
     Places next;
     const auto ahead = [&](Block& b, int at) {              // asks for the block at `at`, whose pages are known, and for the pages of the one behind
         const Places now = next;                            // (whether or not there is one: what is asked for twice is the last key)
-        next = look_up_block(at + 128);
+        next = look_up_block(at + STEP);
         issue(b, now, at);
     };
     Block one;
     if (kb < ke) {
         next = look_up_block(kb);
         ahead(one, kb);
-        if constexpr (RT == 1) {                            // few rows: two blocks, one on its way while the other is used
+        if constexpr (S::kTwo) {
             Block two;
             for (;;) {
-                ahead(two, kb + 128);
+                ahead(two, kb + STEP);
                 __builtin_amdgcn_sched_barrier(0);
                 consume(one, kb, [] {});
                 __builtin_amdgcn_sched_barrier(0);
-                if ((kb += 128) >= ke) break;
-                ahead(one, kb + 128);
+                if ((kb += STEP) >= ke) break;
+                ahead(one, kb + STEP);
                 __builtin_amdgcn_sched_barrier(0);
                 consume(two, kb, [] {});
                 __builtin_amdgcn_sched_barrier(0);
-                if ((kb += 128) >= ke) break;
+                if ((kb += STEP) >= ke) break;
             }
         } else {
-            for (; kb < ke; kb += 128) consume(one, kb, [&] { ahead(one, kb + 128); });
+            for (; kb < ke; kb += STEP) consume(one, kb, [&] { ahead(one, kb + STEP); });
         }
     }
 
@@ -495,8 +532,9 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 template <typename TQ, typename TC, int HDP, int RT>
 constexpr int tile_lds() {
     constexpr int kTurn = 4 * 16 * RT * (16 * turn_subtiles<RT>() + 4) * 4;
-    return (9 * 16 * RT + (sizeof(TC) == 1 ? 256 : 0)) * 4 +
-           (4 * Values<TC, HDP>::kBytes > kTurn ? 4 * Values<TC, HDP>::kBytes : kTurn);
+    constexpr int NU = Shape<TQ, TC, HDP, RT>::NU;
+    return (9 * 16 * RT + (sizeof(TC) == 1 ? 8 * 16 * NU : 0)) * 4 +
+           (4 * Values<TC, HDP, NU>::kBytes > kTurn ? 4 * Values<TC, HDP, NU>::kBytes : kTurn);
 }
 
 // Workgroups: key head fastest (a head's workgroups share its keys and, dealt out in turn, an XCD's L2), then splits, then

@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -73,7 +74,7 @@ def _lib():
         lib.st_sample_filtered.argtypes = [_c_p, _c_p, _c_i64, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]
         lib.st_quant_kv_write.argtypes = [_c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p] + [_c_int] * 8 + [_c_p]
         lib.st_quant_kv_read.argtypes = [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p] + [_c_int] * 8 + [_c_p]
-        lib.st_tile_attention.argtypes = [_c_p, _c_p]
+        lib.st_tile_attention.argtypes = [ctypes.c_char_p, _c_p]
         lib.st_token_conv.argtypes = [_c_p, _c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_p]
         lib.st_token_conv_state.argtypes = [_c_p, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int,
@@ -245,14 +246,31 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True) -
         raise KernelError(f"{name} must be contiguous")
 
 
-def _on_one_device(*tensors: Optional[torch.Tensor]) -> None:
-    """Refuses tensors that are not all on the current device: the stream is that device's."""
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise KernelError(f"a tensor on {t.device}, the current device is cuda:{here}")
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _here(t: torch.Tensor, name: str) -> int:
+    """The current device's index, which the stream of a call belongs to; refuses a tensor that is on no GPU."""
+    if not t.is_cuda:
+        raise KernelError(f"{name} must be a GPU tensor")
+    here = torch.cuda.current_device() if _get_device is None else _get_device()
     if _device_index is not None and _device_index != here:
         raise KernelError(f"this process launches on cuda:{_device_index}, the current device is cuda:{here}")
+    return here
+
+
+def _all_fit(here: int, dtype, shape, **tensors: torch.Tensor) -> None:
+    """``_need`` for tensors of one type and shape, which have to be on the device ``here``."""
+    for name, t in tensors.items():
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != here:
+            _need(t, name, dtype, shape)
+            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{here}")
+
+
+def _at(here: int, t: torch.Tensor, name: str) -> None:
+    if t.get_device() != here:
+        _need(t, name, contiguous=False)
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{here}")
 
 
 # ------------------------------------------------------------------------ lookup
@@ -805,17 +823,25 @@ def prefill_available() -> bool:
 QUANT = torch.float8_e4m3fn      # the entries' type; an entry is worth e4m3 * 2^(exponent - 127)
 
 
-def _quant_cache(k_cache, v_cache, k_exp, v_exp):
+def _quant_cache(here, k_cache, v_cache, k_exp, v_exp):
     """Sizes of an 8-bit cache after checking it: (pages, heads, page size, head size, page stride, exponents' page stride)."""
-    if k_cache.dim() != 4:
+    shape = k_cache.shape
+    if len(shape) != 4:
         raise KernelError("k_cache must have shape [pages, heads, page size, head size]")
-    num_pages, nkv, ps, hd = k_cache.shape
+    num_pages, nkv, ps, hd = shape
+    exps = (num_pages, nkv, ps)
+    if (k_cache.dtype is QUANT and v_cache.dtype is QUANT and v_cache.shape == shape and k_exp.dtype is torch.uint8 and v_exp.dtype is torch.uint8
+            and k_exp.shape == exps and v_exp.shape == exps and k_cache.is_contiguous() and v_cache.is_contiguous() and k_exp.is_contiguous()
+            and v_exp.is_contiguous() and k_cache.get_device() == v_cache.get_device() == k_exp.get_device() == v_exp.get_device() == here):
+        return num_pages, nkv, ps, hd, nkv * ps * hd, nkv * ps
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _need(c, name, QUANT, (num_pages, nkv, ps, hd), contiguous=False)
+        _need(c, name, QUANT, shape, contiguous=False)
+        _at(here, c, name)
         if c.stride()[1:] != (ps * hd, hd, 1):
             raise KernelError(f"{name}: a page must be contiguous")
     for name, e in (("k_exp", k_exp), ("v_exp", v_exp)):
-        _need(e, name, torch.uint8, (num_pages, nkv, ps), contiguous=False)
+        _need(e, name, torch.uint8, exps, contiguous=False)
+        _at(here, e, name)
         if e.stride()[1:] != (ps, 1):
             raise KernelError(f"{name}: a page must be contiguous")
     if k_cache.stride(0) != v_cache.stride(0) or k_exp.stride(0) != v_exp.stride(0):
@@ -838,27 +864,32 @@ def quant_kv_write(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Te
     smallest exponent with which the largest finite magnitude is at most 448 (127 for a head of zeros).  What is not finite becomes NaN.
     k_src/v_src: [T, num_kv_heads*head_dim] views with a common row stride, float32 or bfloat16.  A token without an item or a position, or whose page
     is none of the pool's, is left out; a (item, position) pair may come once in a call."""
-    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+    here = _here(k_cache, "k_cache")
+    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(here, k_cache, v_cache, k_exp, v_exp)
     if ps != page_size:
         raise KernelError(f"cache pages hold {ps} tokens, the step says {page_size}")
-    T = k_src.shape[0]
-    for name, s in (("k_src", k_src), ("v_src", v_src)):
-        _need(s, name, k_src.dtype, (T, nkv * hd), contiguous=False)
-        if s.stride(1) != 1 or s.stride(0) != k_src.stride(0):
-            raise KernelError(f"{name}: rows must be dense with a common stride")
-    _need(token_item, "token_item", torch.int32, (T,))
-    _need(positions, "positions", torch.int32, (T,))
-    _need_table(block_table)
-    _on_one_device(k_cache, v_cache, k_exp, v_exp, k_src, v_src, token_item, positions, block_table)
-    _check(_lib().st_quant_kv_write(_ptr(k_cache), _ptr(v_cache), stride, _ptr(k_exp), _ptr(v_exp), exp_stride, _ptr(k_src), _ptr(v_src),
-                                    k_src.stride(0) if T > 1 else nkv * hd, _ptr(token_item), _ptr(positions), _ptr(block_table),
-                                    block_table.shape[0], block_table.shape[1], ps, num_pages, T, nkv, hd, dtype_code(k_src.dtype), _stream()))
+    T, width = k_src.shape[0], nkv * hd
+    row = k_src.stride()
+    if k_src.shape != (T, width) or v_src.shape != (T, width) or v_src.dtype is not k_src.dtype or row[1] != 1 or v_src.stride() != row:
+        for name, s in (("k_src", k_src), ("v_src", v_src)):
+            _need(s, name, k_src.dtype, (T, width), contiguous=False)
+        raise KernelError("k_src, v_src: rows must be dense with a common stride")
+    _at(here, k_src, "k_src")
+    _at(here, v_src, "v_src")
+    _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions)
+    items, pages = _need_table(here, block_table)
+    _check(_lib().st_quant_kv_write(k_cache.data_ptr(), v_cache.data_ptr(), stride, k_exp.data_ptr(), v_exp.data_ptr(), exp_stride, k_src.data_ptr(),
+                                    v_src.data_ptr(), row[0] if T > 1 else width, token_item.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
+                                    items, pages, ps, num_pages, T, nkv, hd, dtype_code(k_src.dtype), _stream()))
 
 
-def _need_table(block_table: torch.Tensor) -> None:
-    _need(block_table, "block_table", torch.int32)
-    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+def _need_table(here: int, block_table: torch.Tensor) -> Tuple[int, int]:
+    """Items and pages an item of a block table."""
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
         raise KernelError("block_table must have shape [items, pages]")
+    _all_fit(here, torch.int32, shape, block_table=block_table)
+    return shape[0], shape[1]
 
 
 def _d_quant_kv_read(k_cache, v_cache, k_exp, v_exp, token_item, positions, block_table, dtype):
@@ -872,18 +903,18 @@ def quant_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Ten
                   positions: torch.Tensor, block_table: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that the 8-bit cache holds for tokens (their items and positions, int32 [T]): two tensors
     [T, num_kv_heads*head_dim] of ``dtype``, exact in bfloat16 as in float32.  Zeros for a token that ``quant_kv_write`` would leave out."""
-    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+    here = _here(k_cache, "k_cache")
+    num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(here, k_cache, v_cache, k_exp, v_exp)
     T = token_item.shape[0]
-    _need(token_item, "token_item", torch.int32, (T,))
-    _need(positions, "positions", torch.int32, (T,))
-    _need_table(block_table)
-    _on_one_device(k_cache, v_cache, k_exp, v_exp, token_item, positions, block_table)
+    _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions)
+    items, pages = _need_table(here, block_table)
     code = dtype_code(dtype)
-    k, v = (empty((T, nkv * hd), dtype, k_cache.device) for _ in range(2))
-    _check(_lib().st_quant_kv_read(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), stride, _ptr(k_exp), _ptr(v_exp), exp_stride, _ptr(token_item),
-                                   _ptr(positions), _ptr(block_table), block_table.shape[0], block_table.shape[1], ps, num_pages, T, nkv, hd,
-                                   code, _stream()))
-    return k, v
+    both = empty((2, T, nkv * hd), dtype, k_cache.device)
+    at = both.data_ptr()
+    _check(_lib().st_quant_kv_read(at, at + T * nkv * hd * both.element_size(), k_cache.data_ptr(), v_cache.data_ptr(), stride, k_exp.data_ptr(),
+                                   v_exp.data_ptr(), exp_stride, token_item.data_ptr(), positions.data_ptr(), block_table.data_ptr(), items, pages,
+                                   ps, num_pages, T, nkv, hd, code, _stream()))
+    return both[0], both[1]
 
 
 # ------------------------------------------- attention of rows that read the same keys
@@ -898,6 +929,10 @@ class _TileAttention(ctypes.Structure):
                [("scale", _c_f)] + [(n, _c_int) for n in ("own_splits", "shared_splits", "slots", "dtype", "cache_dtype", "shared_entries")]
 
 
+# the same as bytes, which takes a fifth of the time of filling in the structure's fields
+_pack_tiles = struct.Struct("@23q13if6i").pack
+
+
 @functools.lru_cache(maxsize=None)
 def _compute_units(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
@@ -905,54 +940,56 @@ def _compute_units(device: int) -> int:
 
 def tile_splits(workgroups: int, max_keys: int, units: int) -> int:
     """Parts that the keys are split into, for ``workgroups`` without a split."""
-    return max(1, min(-(-2 * units // max(1, workgroups)), max_keys // 128, 32))
+    groups = max(1, workgroups)
+    return max(1, min(-(-units // groups), max_keys // 256, 32), min(3 * units // groups, max_keys // 1024, 32))
 
 
-def _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, own_splits, shared_splits, out, workspace, **lists):
-    """Checks what all faces of the kernel share and launches it; ``rows``: rows of the partial results."""
+def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, own_splits, shared_splits, out, workspace, *,
+                    token_item=0, positions=0, row_ids=0, tile_item=0, tile_q0=0, item_tok_off=0, item_start=0, item_len=0, row_start=0,
+                    shared_rows=0, group_off=0, num_entries=0, num_tiles=0, tile_rows=0, num_shared=0, num_groups=0):
+    """Checks what all faces of the kernel share and launches it.  ``rows``: rows of the partial results; the lists are addresses."""
     quant = k_exp is not None
     if quant:
-        num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(k_cache, v_cache, k_exp, v_exp)
+        num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(here, k_cache, v_cache, k_exp, v_exp)
     else:
         num_pages, nkv, ps, hd = _check_cache(k_cache, v_cache, q)
         stride, exp_stride = k_cache.stride(0), 0
-    T = q.shape[0]
+        _at(here, k_cache, "k_cache")
+        _at(here, v_cache, "v_cache")
+    T, width = q.shape
     if num_q_heads < 1 or num_q_heads % nkv:
         raise KernelError(f"{num_q_heads} query heads do not divide into {nkv} key heads")
     code = dtype_code(q.dtype)
-    _need(q, "q", None, (T, num_q_heads * hd), contiguous=False)
-    if q.stride(1) != 1:
+    row = q.stride()
+    if width != num_q_heads * hd or row[1] != 1 or q.get_device() != here:
+        _need(q, "q", None, (T, num_q_heads * hd), contiguous=False)
+        _at(here, q, "q")
         raise KernelError("q rows must be dense")
-    _need_table(block_table)
+    items, pages = _need_table(here, block_table)
+    if out is None:
+        out = empty((T, width), q.dtype, q.device)
+    else:
+        _all_fit(here, q.dtype, (T, width), out=out)
     slots = own_splits + shared_splits
     if slots > 64:
         raise KernelError(f"attention: {slots} parts of the keys (at most 64)")
-    part_o = part_lse = None
+    part_o = part_lse = 0
     if slots > 1:
         n_l = rows * num_q_heads * slots
         if workspace is None:
             workspace = empty((n_l * (hd + 1),), torch.float32, q.device)
-        _need(workspace, "workspace", torch.float32)
-        if workspace.numel() < n_l * (hd + 1):
-            raise KernelError("attention workspace is too small")
-        part_o = _ptr(workspace)
+        else:
+            _need(workspace, "workspace", torch.float32)
+            _at(here, workspace, "workspace")
+            if workspace.numel() < n_l * (hd + 1):
+                raise KernelError("attention workspace is too small")
+        part_o = workspace.data_ptr()
         part_lse = part_o + 4 * n_l * hd
-    _on_one_device(q, k_cache, v_cache, k_exp, v_exp, block_table, out, workspace, *(t for t in lists.values() if isinstance(t, torch.Tensor)))
-    args = _TileAttention(out=_ptr(out), part_o=part_o, part_lse=part_lse, q=_ptr(q), q_stride=q.stride(0) if T > 1 else num_q_heads * hd,
-                          k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), page_stride=stride, k_exp=_ptr(k_exp), v_exp=_ptr(v_exp),
-                          exp_stride=exp_stride, block_table=_ptr(block_table), num_rows=T, num_items=block_table.shape[0],
-                          max_pages=block_table.shape[1], page_size=ps, num_pages=num_pages, heads=num_q_heads, kv_heads=nkv, head_dim=hd,
-                          scale=float(scale), own_splits=own_splits, shared_splits=shared_splits, slots=slots, dtype=code,
-                          cache_dtype=2 if quant else code,
-                          **{n: _ptr(t) if isinstance(t, torch.Tensor) else t for n, t in lists.items() if t is not None})
-    _check(_lib().st_tile_attention(ctypes.byref(args), _stream()))
-    return out
-
-
-def _tile_out(q, out, width):
-    if out is None:
-        out = empty((q.shape[0], width), q.dtype, q.device)
-    _need(out, "out", q.dtype, (q.shape[0], width))
+    _check(_lib().st_tile_attention(_pack_tiles(
+        out.data_ptr(), part_o, part_lse, q.data_ptr(), row[0] if T > 1 else width, k_cache.data_ptr(), v_cache.data_ptr(), stride,
+        k_exp.data_ptr() if quant else 0, v_exp.data_ptr() if quant else 0, exp_stride, token_item, positions, block_table.data_ptr(), row_ids,
+        tile_item, tile_q0, item_tok_off, item_start, item_len, row_start, shared_rows, group_off, T, num_entries, num_tiles, tile_rows, num_shared,
+        num_groups, items, pages, ps, num_pages, num_q_heads, nkv, hd, scale, own_splits, shared_splits, slots, code, 2 if quant else code, 0), _stream()))
     return out
 
 
@@ -976,19 +1013,17 @@ def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     are skipped) only those batch rows are computed and written.  A row without an item or a position gets zeros.  ``max_keys``: the most keys that
     a row reads, for the choice of ``num_splits`` where that is 0 (default: what the block table can hold); results do not need it to
     be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 1)."""
-    T, hd = q.shape[0], k_cache.shape[-1]
-    _need(token_item, "token_item", torch.int32, (T,))
-    _need(positions, "positions", torch.int32, (T,))
+    here = _here(q, "q")
+    T = q.shape[0]
+    _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions)
+    rows, ids = T, 0
     if row_ids is not None:
-        _need(row_ids, "row_ids", torch.int32, (row_ids.shape[0],))
-    rows = T if row_ids is None else row_ids.shape[0]
-    out = _tile_out(q, out, num_q_heads * hd)
-    if rows == 0:
-        return out
+        rows, ids = row_ids.shape[0], row_ids.data_ptr()
+        _all_fit(here, torch.int32, (rows,), row_ids=row_ids)
     if num_splits <= 0:
-        num_splits = tile_splits(rows * k_cache.shape[1], _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(q.device.index))
-    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, int(num_splits), 0, out, workspace,
-                           token_item=token_item, positions=positions, row_ids=row_ids, num_entries=rows)
+        num_splits = tile_splits(rows * k_cache.shape[1], _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(here))
+    return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, num_splits, 0, out, workspace,
+                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_ids=ids, num_entries=rows)
 
 
 @_timed("attention_prefill_quant", _d_attention_quant)
@@ -1001,23 +1036,19 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     [tile_q0[i], tile_q0[i]+tile_rows) of item tile_item[i] (-1: none); row r of an item sits at batch row item_tok_off[item]+r and at position
     item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
     ``attention_rows_quant``."""
-    hd, nt = k_cache.shape[-1], tile_item.shape[0]
-    _need(tile_item, "tile_item", torch.int32, (nt,))
-    _need(tile_q0, "tile_q0", torch.int32, (nt,))
-    for name, v in (("item_tok_off", item_tok_off), ("item_start", item_start), ("item_len", item_len)):
-        _need(v, name, torch.int32, (block_table.shape[0],))
+    here = _here(q, "q")
+    nt = tile_item.shape[0]
+    _all_fit(here, torch.int32, (nt,), tile_item=tile_item, tile_q0=tile_q0)
+    _all_fit(here, torch.int32, (block_table.shape[0],), item_tok_off=item_tok_off, item_start=item_start, item_len=item_len)
     if tile_rows < 1 or tile_rows > 65536:
         raise KernelError(f"tiles of {tile_rows} rows")
-    out = _tile_out(q, out, num_q_heads * hd)
-    if nt == 0 or q.shape[0] == 0:
-        return out
+    nkv = k_cache.shape[1]
     if num_splits <= 0:
-        group = max(1, num_q_heads // k_cache.shape[1])
-        num_splits = tile_splits(nt * k_cache.shape[1] * max(1, tile_rows * group // 64), _key_bound(max_keys, block_table, k_cache.shape[2]),
-                                 _compute_units(q.device.index))
-    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, q.shape[0], int(num_splits), 0, out, workspace,
-                           tile_item=tile_item, tile_q0=tile_q0, item_tok_off=item_tok_off, item_start=item_start, item_len=item_len,
-                           num_tiles=nt, tile_rows=int(tile_rows))
+        num_splits = tile_splits(nt * nkv * max(1, tile_rows * (num_q_heads // nkv) // 64), _key_bound(max_keys, block_table, k_cache.shape[2]),
+                                 _compute_units(here))
+    return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, q.shape[0], num_splits, 0, out, workspace,
+                           tile_item=tile_item.data_ptr(), tile_q0=tile_q0.data_ptr(), item_tok_off=item_tok_off.data_ptr(),
+                           item_start=item_start.data_ptr(), item_len=item_len.data_ptr(), num_tiles=nt, tile_rows=tile_rows)
 
 
 def _d_attention_shared(q, k_cache, v_cache, *a, **kw):
@@ -1040,29 +1071,24 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
     ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 1)."""
-    T, hd = q.shape[0], k_cache.shape[-1]
+    here = _here(q, "q")
+    T = q.shape[0]
     if (k_exp is None) != (v_exp is None):
         raise KernelError("an 8-bit cache has exponents of keys and of values")
-    for name, v in (("token_item", token_item), ("positions", positions), ("row_start", row_start)):
-        _need(v, name, torch.int32, (T,))
-    _need(shared_rows, "shared_rows", torch.int32, (shared_rows.shape[0],))
-    _need(group_off, "group_off", torch.int32, (group_off.shape[0],))
-    groups, n = group_off.shape[0] - 1, shared_rows.shape[0]
+    _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions, row_start=row_start)
+    n, groups = shared_rows.numel(), group_off.numel() - 1
     if groups < 1 or n < 1:
         raise KernelError("attention_shared needs a group of rows (attention_rows and attention_rows_quant serve a batch without one)")
-    out = _tile_out(q, out, num_q_heads * hd)
-    if T == 0:
-        return out
-    nkv, units = k_cache.shape[1], _compute_units(q.device.index)
-    group = max(1, num_q_heads // nkv)
+    _all_fit(here, torch.int32, (n,), shared_rows=shared_rows)
+    _all_fit(here, torch.int32, (groups + 1,), group_off=group_off)
+    nkv, ps, units = k_cache.shape[1], k_cache.shape[2], _compute_units(here)
     if shared_splits <= 0:
-        tiles = max(groups, n * group // 64)
-        shared_splits = tile_splits(tiles * nkv, _key_bound(max_shared, block_table, k_cache.shape[2]), units)
+        shared_splits = tile_splits(max(groups, n * (num_q_heads // nkv) // 64) * nkv, _key_bound(max_shared, block_table, ps), units)
     if own_splits <= 0:
-        own_splits = tile_splits(T * nkv, _key_bound(max_own, block_table, k_cache.shape[2]), units)
-    return _tile_attention(q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, T, int(own_splits), int(shared_splits), out, workspace,
-                           token_item=token_item, positions=positions, row_start=row_start, shared_rows=shared_rows, group_off=group_off,
-                           num_entries=T, num_shared=n, num_groups=groups)
+        own_splits = tile_splits(T * nkv, _key_bound(max_own, block_table, ps), units)
+    return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, T, own_splits, shared_splits, out, workspace,
+                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_start=row_start.data_ptr(),
+                           shared_rows=shared_rows.data_ptr(), group_off=group_off.data_ptr(), num_entries=T, num_shared=n, num_groups=groups)
 
 
 # ---------------------------------------------------------------------- sampling
@@ -1107,25 +1133,33 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature: t
     logit, lowest index among equals.  Weights are whole numbers of 2^-44 of the largest, so results do not depend on any order
     of summation.  A NaN logit is never chosen unless the row has nothing else.  Up to 2^18 logits a row."""
     R, V = logits.shape
-    _need(logits, "logits", torch.float32, (R, V), contiguous=False)
     if V < 1 or V > 1 << 18:
         raise KernelError(f"sample_filtered takes 1 to {1 << 18} logits a row, not {V}")
-    if logits.stride(1) != 1 and V > 1:
-        raise KernelError("logits: rows must be dense")
-    _need(uniforms, "uniforms", torch.float32, (R,))
-    _need(temperature, "temperature", torch.float32, (R,))
-    for name, t, dt in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if t is not None:
-            _need(t, name, dt, (R,))
+    stride = V
+    if logits.dtype is not torch.float32 or not logits.is_cuda or not logits.is_contiguous():
+        _need(logits, "logits", torch.float32, (R, V), contiguous=False)
+        if logits.stride(1) != 1 and V > 1:
+            raise KernelError("logits: rows must be dense")
+        if R > 1:
+            stride = logits.stride(0)
+            if stride < V:
+                raise KernelError("logits: rows overlap")
+    here = _here(logits, "logits")
+    _at(here, logits, "logits")
+    shape = (R,)
+    _all_fit(here, torch.float32, shape, uniforms=uniforms, temperature=temperature)
+    if top_k is not None:
+        _all_fit(here, torch.int32, shape, top_k=top_k)
+    if top_p is not None:
+        _all_fit(here, torch.float32, shape, top_p=top_p)
+    if min_p is not None:
+        _all_fit(here, torch.float32, shape, min_p=min_p)
     if out is None:
-        out = torch.empty((R,), dtype=torch.int32, device=logits.device)
-    _need(out, "out", torch.int32, (R,))
-    _on_one_device(logits, uniforms, temperature, top_k, top_p, min_p, out)
-    stride = max(logits.stride(0), V) if R > 1 else V
-    if R > 1 and logits.stride(0) < V:
-        raise KernelError("logits: rows overlap")
-    _check(_lib().st_sample_filtered(_ptr(out), _ptr(logits), stride, R, V, _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                     _ptr(min_p), _stream()))
+        out = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    else:
+        _all_fit(here, torch.int32, shape, out=out)
+    _check(_lib().st_sample_filtered(out.data_ptr(), logits.data_ptr(), stride, R, V, uniforms.data_ptr(), temperature.data_ptr(), _ptr(top_k),
+                                     _ptr(top_p), _ptr(min_p), _stream()))
     return out
 
 

@@ -53,18 +53,28 @@ def test_tile_attention():
     ok = dict(out=p, part_o=p, part_lse=p, q=p, q_stride=256, k_cache=p, v_cache=p, page_stride=2 * 16 * 64, k_exp=p, v_exp=p, exp_stride=32, token_item=p,
               positions=p, block_table=p, num_rows=0, num_entries=0, num_items=1, max_pages=4, page_size=16, num_pages=9, heads=4, kv_heads=2, head_dim=64,
               scale=1.0, own_splits=1, slots=1, dtype=1, cache_dtype=2)
-    call = lambda **kw: lib.st_tile_attention(ctypes.byref(K._TileAttention(**{**ok, **kw})), None)  # noqa: E731
+    call = lambda **kw: lib.st_tile_attention(bytes(K._TileAttention(**{**ok, **kw})), None)  # noqa: E731
     assert call() == 0
+    one = dict(num_rows=1, num_entries=1)
     shared = dict(row_start=p, shared_rows=p, group_off=p, num_groups=1, num_shared=2, shared_splits=1, slots=2)
     for bad, says in ((dict(heads=5), "divide"), (dict(head_dim=40), "multiple of 16"), (dict(head_dim=512), "multiple of 16"), (dict(page_size=0), "bad sizes"),
                       (dict(num_items=0), "bad sizes"), (dict(max_pages=1 << 28), "2^31"), (dict(dtype=7), "dtype"), (dict(cache_dtype=0), "cache of type"),
                       (dict(cache_dtype=1), "kernels of their own"), (dict(k_exp=None), "exponents"), (dict(exp_stride=3), "exponents"),
                       (dict(page_stride=1024), "page stride"), (dict(page_stride=2 * 16 * 64 + 8), "page stride"), (dict(page_stride=1 << 32), "page stride"),
                       (dict(own_splits=0, slots=0), "splits"), (dict(own_splits=70, slots=70), "splits"), (dict(own_splits=2, slots=1), "splits"),
-                      (dict(own_splits=2, slots=2, part_o=None), "null"), (dict(q=None), "null"), (dict(q=4104), "aligned"), (dict(q_stride=257), "aligned"),
+                      (dict(one, own_splits=2, slots=2, part_o=None), "null"), (dict(one, q=None), "null"), (dict(one, q=4104), "aligned"),
+                      (dict(one, q_stride=257), "aligned"), (dict(one, out=None), "null"),
                       (dict(num_tiles=1, tile_rows=64), "tiles need"), (dict(shared, row_start=None), "lists"), (dict(shared, shared_splits=0, slots=1), "splits"),
                       (dict(shared, row_ids=p), "lists")):
         assert says in error(call(**bad)), bad
+
+
+def test_packed_arguments_are_the_structure():
+    """Every field in its place: numbers that say which one they are."""
+    n = len(K._TileAttention._fields_)
+    values = list(range(1, n + 1))
+    assert K._pack_tiles(*values) == bytes(K._TileAttention(*values))[:len(K._pack_tiles(*values))]
+    assert len(bytes(K._TileAttention())) - len(K._pack_tiles(*values)) < 8      # (padding at the end)
 
 
 def test_faces_want_gpu_tensors():
