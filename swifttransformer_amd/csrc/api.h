@@ -171,6 +171,7 @@ struct StTileAttention {
     int heads, kv_heads, head_dim;
     float scale;
     int own_splits, shared_splits, slots, dtype, cache_dtype;
+    int own_waves;              // waves that share a row's keys (not a tile's or a group's): 4, or 1, four rows a workgroup then
     int shared_entries;         // (the library's own)
 };
 int st_tile_attention(const StTileAttention* args, hipStream_t stream);

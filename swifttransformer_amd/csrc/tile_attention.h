@@ -114,10 +114,10 @@ template <int RT> constexpr int turn_subtiles() { return RT == 1 ? 4 : RT == 2 ?
 
 // Subtiles of 16 keys a block, and whether two blocks are held, one on its way while the other is used (where the registers do for that).
 template <typename TQ, typename TC, int HDP, int RT> struct Shape {
-    static constexpr int NU = RT == 1 && HDP == 2 ? 4 : 2;
+    static constexpr int NU = 2;
     static constexpr int NV = (2 * HDP * (int)sizeof(TC) + 3) / 4;             // 16-byte chunks of a value that a lane moves (four lanes a value)
     static constexpr int kBlock = NU * (HDP * (int)sizeof(Raw8<TC>) / 4 + 4 * NV);
-    static constexpr bool kTwo = 2 * kBlock + RT * (HDP * (int)sizeof(Op8<TQ>) / 4 + 8 * HDP + 8 * NU) <= 416;
+    static constexpr bool kTwo = 2 * kBlock + RT * (HDP * (int)sizeof(Op8<TQ>) / 4 + 8 * HDP + 8 * NU) <= 200;
 };
 
 constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
@@ -131,6 +131,7 @@ struct TileWork {
     int base;              // the token; the item's first batch row; the list's first place
     int start;             // kinds 0 and 1: position of the first row's token
     int slot, splits, split;
+    int waves;             // 4 share the keys, or 1 has them alone (the others work on other rows)
 };
 
 // flat row j's token and how many keys it sees; -1 where there is none
@@ -167,10 +168,11 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     constexpr bool QUANT = sizeof(TC) == 1;
     constexpr int ES = sizeof(TC);
     using S = Shape<TQ, TC, HDP, RT>;
-    constexpr int NU = S::NU, NV = S::NV, KEYS = 16 * NU, STEP = 4 * KEYS, NF = NU / 2;
+    constexpr int NU = S::NU, NV = S::NV, KEYS = 16 * NU, NF = NU / 2;
     constexpr int VB = Values<TC, HDP, NU>::kBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r16 = lane & 15;
+    const int STEP = w.waves * KEYS;                        // keys between a wave's blocks
     const int G = p.heads / p.kv_heads, hd = p.head_dim, ps = p.page_size;
     float* s_m = reinterpret_cast<float*>(lds);             // [4][R] the waves' maxima
     float* s_l = s_m + 4 * R;                               // [4][R] and normalisers
@@ -201,7 +203,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             if (t < 0 || d >= hd) clear(r);
             to_op(r, qf[rt][s]);
         }
-        if (wave == 0 && g == 0) s_t[16 * rt + r16] = t;
+        if (wave == 0 && g == 0) s_t[16 * rt + r16] = t;     // (read only where the waves share their rows)
         most = max(most, sees);
         lim[rt] = t < 0 ? 0x7fffffff : sees;                // (a row that is none takes whatever comes)
         least = min(least, lim[rt]);
@@ -438,7 +440,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
         }
     };
-    int kb = kb0 + KEYS * wave;
+    int kb = kb0 + (w.waves == 1 ? 0 : KEYS * wave);
     Places next;
     const auto ahead = [&](Block& b, int at) {              // asks for the block at `at`, whose pages are known, and for the pages of the one behind
         const Places now = next;                            // (whether or not there is one: what is asked for twice is the last key)
@@ -466,6 +468,25 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         } else {
             for (; kb < ke; kb += STEP) consume(one, kb, [&] { ahead(one, kb + STEP); });
         }
+    }
+
+    const int place = (w.kind == 2 ? p.own_splits : 0) + w.split;      // of the row's partial results
+    if (RT == 1 && w.waves == 1) {                          // nothing to join: from the registers
+        const float sum = rows4_sum(l[0]), inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const int f = w.first + r16, t = w.base + f / G, head = kvh * G + f - f / G * G;
+        if (f < w.count) {                                  // (kind 0: one token, which is there)
+            const int64_t at = (int64_t)(w.slot >= 0 ? w.slot : t) * p.heads + head;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const int d = 16 * dt + 4 * g;
+                if (16 * dt >= hd) break;
+                const float res[4] = {acc[0][dt][0] * inverse, acc[0][dt][1] * inverse, acc[0][dt][2] * inverse, acc[0][dt][3] * inverse};
+                if (p.slots == 1) Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + d, res);
+                else Elem<float>::store4(p.part_o + (at * p.slots + place) * hd + d, res);
+            }
+            if (p.slots > 1 && g == 0) p.part_lse[at * p.slots + place] = sum == 0.f ? -INFINITY : m[0] + log2f(sum);
+        }
+        return;
     }
 
     // ---- the waves' results, joined
@@ -520,12 +541,12 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             if (p.slots == 1)
                 Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + d, res);
             else
-                Elem<float>::store4(p.part_o + (out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split) * hd + d, res);
+                Elem<float>::store4(p.part_o + (out_row * p.slots + place) * hd + d, res);
         }
         if (d0 + DC < DT) __syncthreads();
     }
     if (t >= 0 && p.slots > 1 && quad == 0)
-        p.part_lse[out_row * p.slots + (w.kind == 2 ? p.own_splits : 0) + w.split] = sum == 0.f ? -INFINITY : top + log2f(sum);
+        p.part_lse[out_row * p.slots + place] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
 // LDS of a workgroup
@@ -549,6 +570,7 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
     TileWork w;
     w.start = w.lo = 0;
     w.slot = -1;
+    w.waves = 4;
     if constexpr (RTS > 0) {
         if (y < p.shared_entries * p.shared_splits) {
             int e = y / p.shared_splits;
@@ -593,6 +615,11 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
             return;
         }
         y -= p.shared_entries * p.shared_splits;
+    }
+    if (p.own_waves == 1) {                                 // a wave each
+        w.waves = 1;
+        y = 4 * y + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (y >= p.num_entries * ((G + 16 * RT - 1) / (16 * RT)) * p.own_splits) return;
     }
     const int entry = y / p.own_splits;
     w.split = y - entry * p.own_splits;
@@ -679,7 +706,9 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     const int64_t entries = (int64_t)(p.num_tiles > 0 ? p.num_tiles : p.num_entries) * chunks;
     StTileAttention q = p;
     q.shared_entries = RTS > 0 ? (int)((int64_t)p.num_shared * G / (16 * (RTS > 0 ? RTS : 1))) + p.num_groups : 0;
-    const int64_t groups = (entries * p.own_splits + (int64_t)q.shared_entries * p.shared_splits) * p.kv_heads;
+    const int64_t own = p.own_waves == 1 ? (entries * p.own_splits + 3) / 4 : entries * p.own_splits;
+    const int64_t groups = (own + (int64_t)q.shared_entries * p.shared_splits) * p.kv_heads;
+    ST_CHECK(entries * p.own_splits < ((int64_t)1 << 31), "attention: too many rows at once");
     ST_CHECK(groups < ((int64_t)1 << 31), "attention: too many rows at once");
     if (groups == 0) return 0;
     constexpr int lds = lds1 > lds2 ? lds1 : lds2;
@@ -717,7 +746,7 @@ int launch_tiles_by_head(const StTileAttention& p, hipStream_t stream) {
     if (p.head_dim <= 64) return launch_tiles_of<TQ, TC, 2, MAX>(p, stream);
     if (p.head_dim <= 96) return launch_tiles_of<TQ, TC, 3, MAX>(p, stream);
     if (p.head_dim <= 128) return launch_tiles_of<TQ, TC, 4, MAX>(p, stream);
-    return launch_tiles_of<TQ, TC, 8, MAX / 2>(p, stream);
+    return launch_tiles_of<TQ, TC, 8, (MAX > 1 ? MAX / 2 : 1)>(p, stream);
 }
 
 // the sources that hold them: by the queries' type and the cache's

@@ -2,7 +2,7 @@
 #include "tile_attention.h"
 
 namespace st {
-int tile_attention_bf16(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<bf16_t, bf16_t, 4>(p, stream); }
+int tile_attention_bf16(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<bf16_t, bf16_t, 2>(p, stream); }
 }  // namespace st
 
 using namespace st;
@@ -25,6 +25,7 @@ extern "C" int st_tile_attention(const StTileAttention* args, hipStream_t stream
     ST_CHECK(p.num_groups == 0 || (p.row_start && p.shared_rows && p.group_off && p.num_tiles == 0 && !p.row_ids), "attention: shared prefixes need their lists");
     ST_CHECK(p.num_tiles == 0 || (p.tile_rows > 0 && p.tile_rows <= 65536 && p.tile_item && p.tile_q0 && p.item_tok_off && p.item_start && p.item_len),
              "attention: tiles need their lists");
+    ST_CHECK(p.own_waves == 4 || (p.own_waves == 1 && p.num_tiles == 0), "attention: %d waves a row (4, or 1 without tiles)", p.own_waves);
     ST_CHECK(p.own_splits >= 1 && (p.num_groups == 0 ? p.shared_splits == 0 : p.shared_splits >= 1) && p.slots == p.own_splits + p.shared_splits && p.slots <= 64,
              "attention: %d and %d splits of the keys in %d places (at most 64)", p.own_splits, p.shared_splits, p.slots);
     if (p.num_rows == 0 || (p.num_entries == 0 && p.num_tiles == 0)) return 0;

@@ -2,5 +2,5 @@
 #include "tile_attention.h"
 
 namespace st {
-int tile_attention_f32(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<float, float, 2>(p, stream); }
+int tile_attention_f32(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<float, float, 1>(p, stream); }
 }  // namespace st

@@ -2,5 +2,5 @@
 #include "tile_attention.h"
 
 namespace st {
-int tile_attention_f32_quant(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<float, e4m3_t, 2>(p, stream); }
+int tile_attention_f32_quant(const StTileAttention& p, hipStream_t stream) { return launch_tiles_by_head<float, e4m3_t, 1>(p, stream); }
 }  // namespace st

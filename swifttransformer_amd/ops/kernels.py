@@ -926,11 +926,11 @@ class _TileAttention(ctypes.Structure):
                 ("item_len", _c_p), ("row_start", _c_p), ("shared_rows", _c_p), ("group_off", _c_p)] + \
                [(n, _c_int) for n in ("num_rows", "num_entries", "num_tiles", "tile_rows", "num_shared", "num_groups", "num_items", "max_pages",
                                       "page_size", "num_pages", "heads", "kv_heads", "head_dim")] + \
-               [("scale", _c_f)] + [(n, _c_int) for n in ("own_splits", "shared_splits", "slots", "dtype", "cache_dtype", "shared_entries")]
+               [("scale", _c_f)] + [(n, _c_int) for n in ("own_splits", "shared_splits", "slots", "dtype", "cache_dtype", "own_waves", "shared_entries")]
 
 
 # the same as bytes, which takes a fifth of the time of filling in the structure's fields
-_pack_tiles = struct.Struct("@23q13if6i").pack
+_pack_tiles = struct.Struct("@23q13if7i").pack
 
 
 @functools.lru_cache(maxsize=None)
@@ -940,13 +940,12 @@ def _compute_units(device: int) -> int:
 
 def tile_splits(workgroups: int, max_keys: int, units: int) -> int:
     """Parts that the keys are split into, for ``workgroups`` without a split."""
-    groups = max(1, workgroups)
-    return max(1, min(-(-units // groups), max_keys // 256, 32), min(3 * units // groups, max_keys // 1024, 32))
+    return max(1, min(-(-units // max(1, workgroups)), max_keys // 256, 32))
 
 
 def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, own_splits, shared_splits, out, workspace, *,
                     token_item=0, positions=0, row_ids=0, tile_item=0, tile_q0=0, item_tok_off=0, item_start=0, item_len=0, row_start=0,
-                    shared_rows=0, group_off=0, num_entries=0, num_tiles=0, tile_rows=0, num_shared=0, num_groups=0):
+                    shared_rows=0, group_off=0, num_entries=0, num_tiles=0, tile_rows=0, num_shared=0, num_groups=0, own_waves=4):
     """Checks what all faces of the kernel share and launches it.  ``rows``: rows of the partial results; the lists are addresses."""
     quant = k_exp is not None
     if quant:
@@ -989,8 +988,14 @@ def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_
         out.data_ptr(), part_o, part_lse, q.data_ptr(), row[0] if T > 1 else width, k_cache.data_ptr(), v_cache.data_ptr(), stride,
         k_exp.data_ptr() if quant else 0, v_exp.data_ptr() if quant else 0, exp_stride, token_item, positions, block_table.data_ptr(), row_ids,
         tile_item, tile_q0, item_tok_off, item_start, item_len, row_start, shared_rows, group_off, T, num_entries, num_tiles, tile_rows, num_shared,
-        num_groups, items, pages, ps, num_pages, num_q_heads, nkv, hd, scale, own_splits, shared_splits, slots, code, 2 if quant else code, 0), _stream()))
+        num_groups, items, pages, ps, num_pages, num_q_heads, nkv, hd, scale, own_splits, shared_splits, slots, code, 2 if quant else code, own_waves, 0), _stream()))
     return out
+
+
+def tile_waves(rows: int, max_keys: int, units: int) -> int:
+    """Waves that share a row's keys: one where there is a wave for every SIMD without sharing, or where there is a block or two
+    of keys for each of four at most."""
+    return 1 if rows >= 4 * units or max_keys <= 128 else 4
 
 
 def _key_bound(max_keys: int, block_table: torch.Tensor, page_size: int) -> int:
@@ -1020,10 +1025,11 @@ def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if row_ids is not None:
         rows, ids = row_ids.shape[0], row_ids.data_ptr()
         _all_fit(here, torch.int32, (rows,), row_ids=row_ids)
+    bound, units, nkv = _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(here), k_cache.shape[1]
     if num_splits <= 0:
-        num_splits = tile_splits(rows * k_cache.shape[1], _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(here))
+        num_splits = tile_splits(rows * nkv, bound, units)
     return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, num_splits, 0, out, workspace,
-                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_ids=ids, num_entries=rows)
+                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_ids=ids, num_entries=rows, own_waves=tile_waves(rows * nkv * num_splits, bound, units))
 
 
 @_timed("attention_prefill_quant", _d_attention_quant)
@@ -1044,7 +1050,7 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise KernelError(f"tiles of {tile_rows} rows")
     nkv = k_cache.shape[1]
     if num_splits <= 0:
-        num_splits = tile_splits(nt * nkv * max(1, tile_rows * (num_q_heads // nkv) // 64), _key_bound(max_keys, block_table, k_cache.shape[2]),
+        num_splits = tile_splits(nt * nkv * max(1, tile_rows * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16)), _key_bound(max_keys, block_table, k_cache.shape[2]),
                                  _compute_units(here))
     return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, q.shape[0], num_splits, 0, out, workspace,
                            tile_item=tile_item.data_ptr(), tile_q0=tile_q0.data_ptr(), item_tok_off=item_tok_off.data_ptr(),
@@ -1083,12 +1089,14 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _all_fit(here, torch.int32, (groups + 1,), group_off=group_off)
     nkv, ps, units = k_cache.shape[1], k_cache.shape[2], _compute_units(here)
     if shared_splits <= 0:
-        shared_splits = tile_splits(max(groups, n * (num_q_heads // nkv) // 64) * nkv, _key_bound(max_shared, block_table, ps), units)
+        shared_splits = tile_splits(max(groups, n * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16)) * nkv, _key_bound(max_shared, block_table, ps), units)
+    own = _key_bound(max_own, block_table, ps)
     if own_splits <= 0:
-        own_splits = tile_splits(T * nkv, _key_bound(max_own, block_table, ps), units)
+        own_splits = tile_splits(T * nkv, own, units)
     return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, T, own_splits, shared_splits, out, workspace,
                            token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_start=row_start.data_ptr(),
-                           shared_rows=shared_rows.data_ptr(), group_off=group_off.data_ptr(), num_entries=T, num_shared=n, num_groups=groups)
+                           shared_rows=shared_rows.data_ptr(), group_off=group_off.data_ptr(), num_entries=T, num_shared=n, num_groups=groups,
+                           own_waves=tile_waves(T * nkv * own_splits, own, units))
 
 
 # ---------------------------------------------------------------------- sampling

@@ -52,7 +52,7 @@ def test_tile_attention():
     p = 4096
     ok = dict(out=p, part_o=p, part_lse=p, q=p, q_stride=256, k_cache=p, v_cache=p, page_stride=2 * 16 * 64, k_exp=p, v_exp=p, exp_stride=32, token_item=p,
               positions=p, block_table=p, num_rows=0, num_entries=0, num_items=1, max_pages=4, page_size=16, num_pages=9, heads=4, kv_heads=2, head_dim=64,
-              scale=1.0, own_splits=1, slots=1, dtype=1, cache_dtype=2)
+              scale=1.0, own_splits=1, slots=1, dtype=1, cache_dtype=2, own_waves=4)
     call = lambda **kw: lib.st_tile_attention(bytes(K._TileAttention(**{**ok, **kw})), None)  # noqa: E731
     assert call() == 0
     one = dict(num_rows=1, num_entries=1)
@@ -64,7 +64,7 @@ def test_tile_attention():
                       (dict(own_splits=0, slots=0), "splits"), (dict(own_splits=70, slots=70), "splits"), (dict(own_splits=2, slots=1), "splits"),
                       (dict(one, own_splits=2, slots=2, part_o=None), "null"), (dict(one, q=None), "null"), (dict(one, q=4104), "aligned"),
                       (dict(one, q_stride=257), "aligned"), (dict(one, out=None), "null"),
-                      (dict(num_tiles=1, tile_rows=64), "tiles need"), (dict(shared, row_start=None), "lists"), (dict(shared, shared_splits=0, slots=1), "splits"),
+                      (dict(num_tiles=1, tile_rows=64), "tiles need"), (dict(own_waves=2), "waves"), (dict(shared, row_start=None), "lists"), (dict(shared, shared_splits=0, slots=1), "splits"),
                       (dict(shared, row_ids=p), "lists")):
         assert says in error(call(**bad)), bad
 
