@@ -58,6 +58,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("-d", "--debug", action="store_true", help="Enable debug mode (print every step)")
     ap.add_argument("--max-new-tokens", type=int, default=128, help="decoding steps per request")
     ap.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
+    ap.add_argument("--top-k", type=int, default=0, help="sample among the k likeliest tokens (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, help="sample among the fewest tokens that hold this much probability (1: all)")
+    ap.add_argument("--min-p", type=float, default=0.0, help="sample among the tokens with this share of the likeliest one's probability (0: all)")
     ap.add_argument("--seed", type=int, default=0, help="seed of the sampler (request i uses seed+i)")
     ap.add_argument("--end-token", type=int, default=None, help="default: config.json's eos_token_id")
     ap.add_argument("--ignore-eos", action="store_true")
@@ -108,7 +111,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     for i, p in enumerate(prompts):
         ids.append(eng.add_request(p, SamplingParams(
             temperature=args.temperature, max_new_tokens=args.max_new_tokens, seed=args.seed + i,
-            eos_token_id=args.end_token, ignore_eos=args.ignore_eos)))
+            eos_token_id=args.end_token, ignore_eos=args.ignore_eos, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)))
     t0 = time.perf_counter()
     done = {}
     while eng.has_work():

@@ -105,6 +105,8 @@ class Engine:
         vocab = self.model.vocab_size
         if any((t < 0 or t >= vocab) for t in prompt):
             raise ValueError(f"prompt token outside [0, {vocab})")
+        if params is not None and params.filtered and vocab > 1 << 18:
+            raise ValueError(f"top_k, top_p and min_p take vocabularies of up to {1 << 18} tokens, not {vocab}")
         req = Request(req_id, [int(t) for t in prompt], params or SamplingParams())
         self.scheduler.add(req)
         self.requests[req_id] = req

@@ -74,6 +74,7 @@ class Sampler:
         cuda = self.device.type == "cuda"
         self._ids_ring = _Ring(None) if cuda else None      # sampled ids on their way back
         self._meta_ring = _Ring(4) if cuda else None        # seeds, counters, temperatures on their way in
+        self._filter_ring = _Ring(None) if cuda else None   # what filtered rows are drawn by
 
     def sample_pending(self, logits: torch.Tensor, params: Sequence[SamplingParams],
                        draws: Sequence[int], best: Optional[torch.Tensor] = None) -> PendingTokens:
@@ -90,23 +91,59 @@ class Sampler:
         if all(p.temperature <= 0 for p in params):
             ids = best if best is not None and best.shape == (R,) else K.sample(logits)
         else:
-            host = np.zeros((R, 4), dtype=np.int32)
-            for i, (p, d) in enumerate(zip(params, draws)):
-                host[i, 0] = np.uint32(p.seed & 0xffffffff).astype(np.int32)
-                host[i, 1] = np.uint32((p.seed >> 32) & 0xffffffff).astype(np.int32)
-                host[i, 2] = np.uint32(d & 0xffffffff).astype(np.int32)
-                host[i, 3] = np.float32(p.temperature).view(np.int32)
-            if self._meta_ring is not None:
-                buf = self._meta_ring.take(R)
-                buf.host[:R] = torch.from_numpy(host)
-                meta = buf.host[:R].to(self.device, non_blocking=True)
-                buf.event.record()
-                buf.busy = True
-            else:
-                meta = torch.from_numpy(host).to(self.device)
-            ids = K.sample(logits, temperature=meta[:, 3].contiguous().view(torch.float32),
-                           seeds=meta[:, 0:2].contiguous(), draws=meta[:, 2].contiguous())
+            filtered = [p.filtered for p in params]
+            if any(filtered):
+                ids = self._filtered(logits, params, draws)
+            if any(p.temperature > 0 and not f for p, f in zip(params, filtered)):
+                plain = self._plain(logits, params, draws)
+                ids = torch.where(self._to_device(np.asarray(filtered, np.int32)) != 0, ids, plain) if any(filtered) else plain
         return PendingTokens(ids, self._ids_ring.take(R) if self._ids_ring is not None else None)
+
+    def _to_device(self, values: np.ndarray) -> torch.Tensor:
+        """int32 values, through a pinned buffer."""
+        if self._filter_ring is None:
+            return torch.from_numpy(values).to(self.device)
+        n = values.shape[0]
+        buf = self._filter_ring.take(n)
+        buf.host[:n] = torch.from_numpy(values)
+        out = buf.host[:n].to(self.device, non_blocking=True)
+        buf.event.record()
+        buf.busy = True
+        return out
+
+    def _plain(self, logits: torch.Tensor, params: Sequence[SamplingParams], draws: Sequence[int]) -> torch.Tensor:
+        """Tokens by temperature alone (greedy where it is 0)."""
+        R = logits.shape[0]
+        host = np.zeros((R, 4), dtype=np.int32)
+        for i, (p, d) in enumerate(zip(params, draws)):
+            host[i, 0] = np.uint32(p.seed & 0xffffffff).astype(np.int32)
+            host[i, 1] = np.uint32((p.seed >> 32) & 0xffffffff).astype(np.int32)
+            host[i, 2] = np.uint32(d & 0xffffffff).astype(np.int32)
+            host[i, 3] = np.float32(p.temperature).view(np.int32)
+        if self._meta_ring is not None:
+            buf = self._meta_ring.take(R)
+            buf.host[:R] = torch.from_numpy(host)
+            meta = buf.host[:R].to(self.device, non_blocking=True)
+            buf.event.record()
+            buf.busy = True
+        else:
+            meta = torch.from_numpy(host).to(self.device)
+        return K.sample(logits, temperature=meta[:, 3].contiguous().view(torch.float32),
+                        seeds=meta[:, 0:2].contiguous(), draws=meta[:, 2].contiguous())
+
+    def _filtered(self, logits: torch.Tensor, params: Sequence[SamplingParams], draws: Sequence[int]) -> torch.Tensor:
+        """Tokens after the requests' filters.  A row's random number is the hash's for an id that no vocabulary has: it depends on
+        the request's seed and its counter, not on the batch."""
+        R = logits.shape[0]
+        values = np.zeros((5, R), dtype=np.float32)         # random number, temperature, k (an integer's bits), p, least share
+        integers = values.view(np.int32)
+        for i, (p, d) in enumerate(zip(params, draws)):
+            values[0, i] = K.hash_uniform(p.seed & 0xffffffff, (p.seed >> 32) & 0xffffffff, d & 0xffffffff, 0xffffffff)
+            values[1, i], values[3, i], values[4, i] = p.temperature, p.top_p, p.min_p
+            integers[2, i] = min(p.top_k, 0x7fffffff)
+        there = self._to_device(integers.reshape(-1)).view(5, R)
+        floats = there.view(torch.float32)
+        return K.sample_filtered(logits, floats[0], floats[1], top_k=there[2], top_p=floats[3], min_p=floats[4])
 
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams],
                draws: Sequence[int]) -> List[int]:
