@@ -12,8 +12,8 @@
 //   top k    the k-th largest of the threads' largest is no larger than the k-th largest of all: a histogram of those 1,024 gives a line
 //            above which little more than k logits lie.  They go to a list in LDS, and what is left to do is done there.
 //   top p    (and a top k above 512) weights (or ones) are summed by 2,048 steps of the value.  The step that holds the border is known
-//            then; if all up to it are few they go to the list, else those of that step, whose keys (value, then index) are divided in LDS until
-//            one is left.  A step with more than 4,096 in it (a row of few values) is divided by passes over the row (cut_order).
+//            then, and from the steps' weights how many there are up to it; if they are few they go to the list, else the pass that sums
+//            weights for the draw leaves out that step and gathers its keys (value, then index), which are divided in LDS until one is left.  A step with more than 4,096 in it (a row of few values) is divided by passes over the row (cut_order).
 //   draw     in the list; or, where many are kept, by sums over the waves' stretches, over lines of 64 of one, over a line.
 #include "api.h"
 #include "common.h"
@@ -39,7 +39,8 @@ __device__ inline uint32_t ordered(float x) {
 struct Shared {
     uint64_t weight[kBins];                           // of a histogram's steps; sums of places
     uint32_t count[kBins];
-    uint64_t wave_sum[16];
+    uint64_t wave_sum[16], stretch[16];
+    float estimate[16];
     uint64_t key[kFew], sorted[kFew];                 // the list: (value's bits, index's complement); weights in an order
     int rank[kFew];
     uint64_t near_key[kNear];                         // keys of the step that holds a border
@@ -461,13 +462,9 @@ __device__ __forceinline__ int draw_from_list(const Row& row, Shared& s, int n, 
     return s.cut.i;
 }
 
-// The token that u draws of all within the cut that weigh at least so much.
-__device__ __forceinline__ int draw_from_row(const Row& row, Shared& s, const Cut cut, double least, float u) {
+// s.stretch: the waves' stretches' sums of the weights within the cut, of those with `least`
+__device__ __forceinline__ void sum_stretches(const Row& row, Shared& s, const Cut cut, double least) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const auto weigh = [&](float x, int i) {
-        const double w = row.weight_whole(x);
-        return within(cut, x, i) & (w >= least) ? w : 0.0;
-    };
     double sum = 0.0;                                 // (of at most 256 weights: exact in 53 bits)
     const auto add = [&](auto plain) {
         row.each<8>([&](const float* x, int i) {
@@ -478,8 +475,9 @@ __device__ __forceinline__ int draw_from_row(const Row& row, Shared& s, const Cu
             double w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (decltype(plain)::value) w[j] = x[j] > cut.v ? row.weight_whole(x[j]) : 0.0;
-                else w[j] = weigh(x[j], i + 64 * j);
+                w[j] = row.weight_whole(x[j]);
+                if constexpr (decltype(plain)::value) w[j] = x[j] > cut.v ? w[j] : 0.0;
+                else w[j] = within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;
             }
             sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         });
@@ -488,15 +486,23 @@ __device__ __forceinline__ int draw_from_row(const Row& row, Shared& s, const Cu
     if (cut.i < 0 && least == 0.0) add(std::true_type());
     else add(std::false_type());
     const uint64_t stretch = wave_sum64(whole(sum));
+    if (lane == 0) s.stretch[wave] = stretch;
     __syncthreads();
-    if (lane == 0) s.wave_sum[wave] = stretch;
-    __syncthreads();
+}
+
+// The token that u draws of all within the cut that weigh at least so much, from s.stretch.
+__device__ __forceinline__ int draw_from_row(const Row& row, Shared& s, const Cut cut, double least, float u) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const auto weigh = [&](float x, int i) {
+        const double w = row.weight_whole(x);
+        return within(cut, x, i) & (w >= least) ? w : 0.0;
+    };
     uint64_t total = 0;
-    for (int w = 0; w < 16; ++w) total += s.wave_sum[w];
+    for (int w = 0; w < 16; ++w) total += s.stretch[w];
     const uint64_t target = drawn_at(u, total);
     uint64_t before = 0;
     int at = 0;
-    for (; at < 15 && before + s.wave_sum[at] < target; ++at) before += s.wave_sum[at];
+    for (; at < 15 && before + s.stretch[at] < target; ++at) before += s.stretch[at];
     // the stretch's lines, a wave every sixteenth
     const int first = at * row.lines * 64;
     for (int j = wave; j < row.lines; j += 64) {
@@ -702,38 +708,100 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
         find_place(s, a, upto, b, share);
         const int bin = (int)s.bin;
         const uint64_t base = s.before;
-        // (all that are to be listed, and perhaps a few more, are not below `line`, and those of the border's step not above `end`)
+        // (all that are kept, and perhaps a few more, are not below `line`, and those of the border's step not above `end`)
         const float line = below_step(bin), end = bin == 0 ? best : best - (float)bin / row.scale * 0.99999f + fabsf(best) * 1e-6f;
-        row.each<8>([&](const float* x, int i) {
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) any |= x[j] >= line;
-            if (!__any(any)) return;
-            if (!full) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) list(x[j], i + 64 * j, (x[j] >= line) & within(cut, x[j], i + 64 * j));
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool in = (x[j] >= line) & (x[j] <= end);
-                if (__any(in)) near(x[j], i + 64 * j, in & within(cut, x[j], i + 64 * j) & (row.step(x[j]) == bin));
-            }
-        });
+        // how many there are up to the border: a step's weight over that of its upper end, too few by a step's width (1.5 %) at most
+        const float one = 5.684341886080802e-14f;     // 2^-44
+        const float falls = (float)row.rate / row.scale;
+        const auto tokens = [&](int step, uint64_t w) { return step <= bin ? (float)w * one * __builtin_amdgcn_exp2f((float)step * falls) : 0.f; };
+        const float some = wave_sum(tokens(2 * threadIdx.x, a) + tokens(2 * threadIdx.x + 1, b));
         __syncthreads();
-        const int n = (int)s.n;
-        if (n <= kFew) {
-            const int token = draw_from_list(row, s, n, n, 1.0, share, least, u);
+        if (lane == 0) s.estimate[wave] = some;
+        __syncthreads();
+        float about = 0.f;
+        for (int w = 0; w < 16; ++w) about += s.estimate[w];
+        if (!(about > (float)kFew)) {
+            row.each<16>([&](const float* x, int i) {
+                bool any = false;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) any |= x[j] >= line;
+                if (!__any(any)) return;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) list(x[j], i + 64 * j, (x[j] >= line) & within(cut, x[j], i + 64 * j));
+            });
+            __syncthreads();
+            const int n = (int)s.n;
+            if (n <= kFew) {
+                const int token = draw_from_list(row, s, n, n, 1.0, share, least, u);
+                if (threadIdx.x == 0) out[r] = token;
+                return;
+            }
+        }
+        // many: the sums over the stretches of all up to the border's step, and the keys of that step, in one pass
+        double sum = 0.0;
+        const auto gather = [&](auto plain) {
+            row.each<8>([&](const float* x, int i) {
+                uint32_t close = 0;
+                bool any = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    close |= (x[j] >= line) & (x[j] <= end) ? 1u << j : 0u;
+                    any |= x[j] >= line;
+                }
+                if (!__any(any)) return;
+                double w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = row.weight_whole(x[j]);
+                    if constexpr (decltype(plain)::value) w[j] = x[j] > end ? w[j] : 0.0;
+                    else w[j] = (x[j] > end) & within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;
+                }
+                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                // those close to the step: a lane's one by one (few lanes have any, hardly one has two)
+                while (__any(close != 0)) {
+                    const int j = __ffs((int)close) - 1;
+                    float y = -INFINITY;
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) y = j == v ? x[v] : y;
+                    const int at = row.step(y);
+                    const bool in = close != 0 && within(cut, y, i + 64 * j);
+                    near(y, i + 64 * j, in & (at == bin));
+                    if (in && at < bin) {
+                        const double own = row.weight_whole(y);
+                        sum += own >= least ? own : 0.0;
+                    }
+                    close &= close - 1;
+                }
+            });
+        };
+        if (cut.i < 0 && least == 0.0) gather(std::true_type());
+        else gather(std::false_type());
+        const uint64_t stretch = wave_sum64(whole(sum));
+        if (lane == 0) s.stretch[wave] = stretch;
+        __syncthreads();
+        if (s.near <= kNear) {
+            const int n = (int)s.near;
+            cut = cut_near<false>(row, s, n, base, share);
+            for (int j = threadIdx.x; j < n; j += 1024) {
+                const uint64_t key = s.near_key[j];
+                const int i = (int)~(uint32_t)key;
+                const uint64_t w = row.weight(value_of(key));
+                if (within(cut, value_of(key), i) && (double)w >= least)
+                    atomicAdd((unsigned long long*)&s.stretch[(i >> 6) / row.lines], (unsigned long long)w);
+            }
+            __syncthreads();
+            const int token = draw_from_row(row, s, cut, least, u);
             if (threadIdx.x == 0) out[r] = token;
             return;
         }
-        if (s.near <= kNear) cut = cut_near<false>(row, s, (int)s.near, base, share);
-        else cut_order<false>(row, s, cut, 0, (double)p);
+        cut_order<false>(row, s, cut, 0, (double)p);
         __syncthreads();
     }
     if (least > 0.0) {
         const Cut c = above(fmaxf(best + t * logf(fminf(min_share, 1.f)) * 1.0001f - 1e-4f * t, row.low));
         if (best < INFINITY && c.v > cut.v) cut = c;
     }
+    sum_stretches(row, s, cut, least);
     const int token = draw_from_row(row, s, cut, least, u);
     if (threadIdx.x == 0) out[r] = token;
 }
