@@ -88,13 +88,13 @@ template <int HDP> __device__ inline void value_op(const char* block, int dt, in
     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(ST_LDS_PTR(short4v, at + 16 * P)));
     o.v = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
 }
-template <int HDP, typename TQ> __device__ inline void value_op(const char* block, int dt, int g, int r16, e4m3_t, Op8<TQ>& o) {
+template <int HDP> __device__ inline Raw8<e4m3_t> value_raw(const char* block, int dt, int g, int r16) {
     constexpr int P = Values<e4m3_t, HDP, 2>::kPitch;
     const int k = r16 >> 1;
     const char* at = block + ((k < 4 ? 4 * g + k : 12 + 4 * g + k)) * P + 16 * dt + 8 * (r16 & 1);
     Raw8<e4m3_t> r;
     r.a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(ST_LDS_PTR(int2v, at)));
-    to_op(r, o);
+    return r;
 }
 template <int HDP> __device__ inline void value_op(const char* block, int dt, int g, int r16, float, Op8<float>& o) {
     constexpr int P = Values<float, HDP, 2>::kPitch;
@@ -260,7 +260,9 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     struct Block {
         Raw8<TC> kr[NU][HDP];
         uint4 vr[NU][NV];
-        uint32_t field[NF];                                 // exponents of the powers of two: lane l's number f is that of key 64 f + l, values behind keys
+        // exponents of the powers of two: WHOLE, of the four keys and values that a lane has scores of in each 16; else lane l's number f is that of
+        // key 64 f + l, values behind keys
+        uint32_t field[WHOLE ? 2 * NU : NF];
         uint64_t bad;                                       // keys whose page is none of the pool's
     };
     const int head_off = kvh * ps * hd;
@@ -292,19 +294,11 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
             if (QUANT) {
 #pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    // (which of the block's 16 keys: a lane's sixteenth of a wave, keys or values)
-                    uint32_t page = q.page[0];
-                    int row = q.row[0], at = kb;
-#pragma unroll
-                    for (int u = 1; u < NU; ++u)
-                        if (((64 * f + lane) % KEYS) >> 4 == u) {
-                            page = q.page[u];
-                            row = q.row[u];
-                            at = kb + 16 * u;
-                        }
-                    const uint8_t* e = 64 * f + lane < KEYS ? p.k_exp : p.v_exp;
-                    b.field[f] = e[(uint64_t)(page < (uint32_t)p.num_pages ? page : 0u) * (uint64_t)p.exp_stride + kvh * ps + row + min(r16, max(ke - 1 - at, 0))];
+                for (int u = 0; u < NU; ++u) {
+                    const uint64_t at = (uint64_t)((uint32_t)q.page[u] < (uint32_t)p.num_pages ? (uint32_t)q.page[u] : 0u) * (uint64_t)p.exp_stride +
+                                        (uint64_t)(kvh * ps + (q.row[u] & ~15));
+                    b.field[2 * u] = *reinterpret_cast<const uint32_t*>(p.k_exp + at + 4 * g);
+                    b.field[2 * u + 1] = *reinterpret_cast<const uint32_t*>(p.v_exp + at + 4 * g);
                 }
             }
         } else {
@@ -346,11 +340,25 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 if ((none >> (16 * u + (lane >> 2))) & 1)
 #pragma unroll
                     for (int c = 0; c < NV; ++c) b.vr[u][c] = make_uint4(0, 0, 0, 0);
+            if constexpr (!WHOLE)
 #pragma unroll
-            for (int f = 0; f < NF; ++f)
-                if ((none >> ((64 * f + lane) % KEYS)) & 1) b.field[f] = 127;
+                for (int f = 0; f < NF; ++f)
+                    if ((none >> ((64 * f + lane) % KEYS)) & 1) b.field[f] = 127;
         }
         const bool whole = kb >= w.lo && kb + KEYS <= min(ke, least) && none == 0;
+        wave_fence();                                       // (the block before has been read)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int at = 16 * (4 * c + (lane & 3));
+                if (64 * NV <= 32 * HDP * ES || at < 32 * HDP * ES)
+                    *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP, NU>::kPitch + at) = b.vr[u][c];
+            }
+        if (QUANT && !WHOLE)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) s_unit[64 * f + lane] = __uint_as_float(b.field[f] << 23);
+        wave_fence();
         floatx4 sc[RT][NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -366,44 +374,47 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
             }
-        wave_fence();                                       // (the block before has been read)
+        // (8-bit values: asked for before the softmax that their trip from LDS takes as long as, where registers are left for them)
+        constexpr bool EARLY = QUANT && HDP <= 4;
+        Raw8<e4m3_t> vraw[EARLY ? DT : 1][NF];
+        if constexpr (EARLY)
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const int at = 16 * (4 * c + (lane & 3));
-                if (64 * NV <= 32 * HDP * ES || at < 32 * HDP * ES)
-                    *reinterpret_cast<uint4*>(s_v + (16 * u + (lane >> 2)) * Values<TC, HDP, NU>::kPitch + at) = b.vr[u][c];
-            }
-        if (QUANT)
-#pragma unroll
-            for (int f = 0; f < NF; ++f) s_unit[64 * f + lane] = __uint_as_float(b.field[f] << 23);
-        then();                                             // (the block's registers are free)
-        wave_fence();
-        floatx4 ku[NU], vu[NU];
+                for (int f = 0; f < NF; ++f) vraw[dt][f] = value_raw<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16);
+        floatx4 ku[NU], vu[NU];                             // powers of two, the keys' with the scale
         if (QUANT) {
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
-                vu[u] = *reinterpret_cast<const floatx4*>(s_unit + KEYS + 16 * u + 4 * g);
+                if constexpr (WHOLE) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        ku[u][r] = __uint_as_float(((b.field[2 * u] >> (8 * r)) & 0xffu) << 23);
+                        vu[u][r] = __uint_as_float(((b.field[2 * u + 1] >> (8 * r)) & 0xffu) << 23);
+                    }
+                } else {
+                    ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
+                    vu[u] = *reinterpret_cast<const floatx4*>(s_unit + KEYS + 16 * u + 4 * g);
+                }
+                ku[u] *= sl;
             }
         }
+        then();                                             // (the block's registers are free)
         float x[RT][4 * NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int i = 0; i < 4 * NU; ++i) {
-                x[rt][i] = sc[rt][i >> 2][i & 3] * sl;
-                if (QUANT) x[rt][i] *= ku[i >> 2][i & 3];
-            }
+            for (int i = 0; i < 4 * NU; ++i) x[rt][i] = sc[rt][i >> 2][i & 3] * (QUANT ? ku[i >> 2][i & 3] : sl);
         if (!whole) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int i = 0; i < 4 * NU; ++i) {
+                const int in = 16 * (i >> 2) + 4 * g + (i & 3), key = kb + in;
+                const bool out = (key >= ke) | (key < w.lo) | ((none >> in) & 1);
 #pragma unroll
-                for (int i = 0; i < 4 * NU; ++i) {
-                    const int in = 16 * (i >> 2) + 4 * g + (i & 3), key = kb + in;
-                    if ((key >= min(ke, lim[rt])) | (key < w.lo) | ((none >> in) & 1)) x[rt][i] = -INFINITY;
-                }
+                for (int rt = 0; rt < RT; ++rt)
+                    if (out | (key >= lim[rt])) x[rt][i] = -INFINITY;
+                if (QUANT && out) vu[i >> 2][i & 3] = 1.f;  // (nothing times whatever lies there)
+            }
         }
         Op8<TQ> pf[RT][NF];
 #pragma unroll
@@ -434,7 +445,9 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
                 Op8<TQ> v;
-                value_op<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16, TC{}, v);
+                if constexpr (EARLY) to_op(vraw[dt][f], v);
+                else if constexpr (QUANT) to_op(value_raw<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16), v);
+                else value_op<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16, TC{}, v);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma8(v, pf[rt][f], acc[rt][dt]);
             }
@@ -725,16 +738,18 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     return 0;
 }
 
-// (Pages that 16 does not divide go by subtiles of 16 rows only.)
+// (Pages that 16 does not divide, or exponents that do not lie at multiples of four, go by subtiles of 16 rows only.)
 template <typename TQ, typename TC, int HDP, int MAX>
 int launch_tiles_of(const StTileAttention& p, hipStream_t stream) {
+    const bool whole = p.page_size % 16 == 0 &&
+                       (sizeof(TC) > 1 || ((reinterpret_cast<uintptr_t>(p.k_exp) | reinterpret_cast<uintptr_t>(p.v_exp) | (uintptr_t)p.exp_stride) & 3) == 0);
     const bool many = (int64_t)p.num_shared * (p.heads / p.kv_heads) > 16 * (int64_t)p.num_groups;
     if (p.num_groups > 0) {
-        if (p.page_size % 16 != 0) return launch_tiles<TQ, TC, HDP, 1, 1, false>(p, stream);
+        if (!whole) return launch_tiles<TQ, TC, HDP, 1, 1, false>(p, stream);
         return many ? launch_tiles<TQ, TC, HDP, 1, MAX, true>(p, stream) : launch_tiles<TQ, TC, HDP, 1, 1, true>(p, stream);
     }
     if constexpr (sizeof(TC) == 1) {
-        if (p.page_size % 16 != 0) return launch_tiles<TQ, TC, HDP, 1, 0, false>(p, stream);
+        if (!whole) return launch_tiles<TQ, TC, HDP, 1, 0, false>(p, stream);
         return p.num_tiles > 0 ? launch_tiles<TQ, TC, HDP, MAX, 0, true>(p, stream) : launch_tiles<TQ, TC, HDP, 1, 0, true>(p, stream);
     }
     ST_CHECK(false, "attention: a cache of the queries' type goes by groups");
