@@ -3,7 +3,7 @@
 //
 // A workgroup takes one key head, up to 16 * RT query rows and a share of the keys.  Query rows are (token, query head of the key head's
 // group) pairs: the heads of one token, of the tokens of a prompt's portion, or of all tokens whose requests begin with the same pages.
-// A key is then read once for all of them.  Its four waves take blocks of 32 or 64 keys in turn, each with a running maximum, normaliser and
+// A key is then read once for all of them.  Its four waves take blocks of 32 keys in turn, each with a running maximum, normaliser and
 // sum of its own (an online softmax in float), and meet in LDS at the end; several workgroups that share a row's keys leave
 // normalised sums and log-sum-exps, which a second kernel joins.
 //
@@ -109,8 +109,8 @@ __device__ inline void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// subtiles of 16 dims that the waves' results are joined by at a time: so many that each thread has a quad of a row's dims (16 rows: 4 subtiles)
-template <int RT> constexpr int turn_subtiles() { return RT == 1 ? 4 : RT == 2 ? 2 : 1; }
+// subtiles of 16 dims that the waves' results are joined by at a time: so many that each thread has a quad of a row's dims
+template <int RT> constexpr int turn_subtiles() { return 4 / RT; }
 
 // Subtiles of 16 keys a block, and whether two blocks are held, one on its way while the other is used (where the registers do for that).
 template <typename TQ, typename TC, int HDP, int RT> struct Shape {
@@ -331,7 +331,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     const float sl = p.scale * 1.44269504088896340736f;     // scores in units of log2
 
     // a block in registers -> maximum, normaliser and sums; `then` is called once its registers are free
-    // (Without branches from the scores' products to the sums: what the compiler knows of a product's result and of loads under way ends at one.)
+    // (What the compiler knows of a product's result and of loads under way ends at a branch: two remain between the products, the mask of a
+    // block that has keys to leave out, and the sums' turn to a new maximum, which most blocks of a long row do without.)
     const auto consume = [&](Block& b, int kb, auto then) {
         const uint64_t none = b.bad;
         if (none != 0) {                                    // (their values are not to be multiplied, not even by nothing)
@@ -617,11 +618,15 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
             w.base = __builtin_amdgcn_readfirstlane(off);
             w.first = __builtin_amdgcn_readfirstlane(e) * R;
             w.count = __builtin_amdgcn_readfirstlane(n) * G;
-            // the block table: that of the first of the group's rows (of the first 64) that has a request
-            const int i = threadIdx.x & 63;
-            const int t = i < n ? p.shared_rows[w.base + i] : -1;
-            const int item = t >= 0 && t < p.num_rows ? p.token_item[t] : -1;
-            const uint64_t there = __ballot((uint32_t)item < (uint32_t)p.num_items);
+            // the block table: that of the first of the group's rows that has a request
+            uint64_t there = 0;
+            int item = -1;
+            for (int base = 0; base < n && !there; base += 64) {
+                const int i = base + (int)(threadIdx.x & 63);
+                const int t = i < n ? p.shared_rows[w.base + i] : -1;
+                item = t >= 0 && t < p.num_rows ? p.token_item[t] : -1;
+                there = __ballot((uint32_t)item < (uint32_t)p.num_items);
+            }
             if (!there) w.lo = 0x7fffffff;                 // none: no key is seen
             w.item = there ? __builtin_amdgcn_readfirstlane(__shfl(item, __ffsll((unsigned long long)there) - 1, 64)) : 0;
             tile_work<TQ, TC, HDP, (RTS > 0 ? RTS : 1), WHOLE>(p, w, kvh, lds);

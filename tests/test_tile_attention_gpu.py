@@ -288,6 +288,23 @@ def test_rows_inside_the_prefix_and_padding_rows():
     compare(got, torch.stack([w for w, _ in want]), torch.stack([b for _, b in want]))
 
 
+@pytest.mark.parametrize("nobody", [63, 64, 150])
+def test_a_group_that_begins_with_many_padding_rows(nobody):
+    """The prefix's pages come from the first row with a request, however far behind in the list it stands."""
+    g = torch.Generator().manual_seed(4)
+    pool, table, lens, start, shared, off, q = shared_batch([(70, 3)], [9], 4, 2, 64, 16, torch.float32, False, g)
+    k, v, _, _ = pool.put()
+    put = lambda x: x.to(DEV)  # noqa: E731
+    rows = [-1] * (nobody - 1) + [3] + list(shared)
+    item = ints([0, 1, 2, -1])
+    got = K.attention_shared(put(torch.cat((q, q[:1]))), k, v, put(item), put(ints([n - 1 for n in lens] + [50])), put(table), 4, 0.125,
+                             put(ints(list(start) + [70])), put(ints(rows)), put(ints([0, len(rows)])), shared_splits=2, own_splits=1)
+    for t, n in enumerate(lens):
+        want, bound = reference(q[t], *pool.entries(table, t, n), 4, 0.125)
+        compare(got[t], want, bound)
+    assert (got[3] == 0).all()
+
+
 def test_a_value_that_is_no_number_reaches_its_rows_only():
     g = torch.Generator().manual_seed(3)
     batch = shared_batch([(70, 4)], [20], 2, 2, 64, 16, torch.bfloat16, False, g)
