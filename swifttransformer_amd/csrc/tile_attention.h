@@ -181,6 +181,11 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     char* s_big = reinterpret_cast<char*>(s_l + 5 * R + (QUANT ? 8 * KEYS : 0));
     char* s_v = s_big + wave * VB;                          // [4][KEYS values], at the end the waves' sums
 
+    // The first of the eight dims that a lane has in product s.  In 8 bits two products' dims lie behind each other, so that a load brings both
+    // (a dot product takes its dims in any order).
+    constexpr bool PAIRS = QUANT && HDP % 2 == 0;
+    const auto dim_of = [&](int s) { return PAIRS ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+
     // ---- query rows
     Op8<TQ> qf[RT][HDP];
     int lim[RT], most = 0, least = 0x7fffffff;
@@ -198,7 +203,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         const TQ* row = (const TQ*)p.q + (int64_t)max(t, 0) * p.q_stride + (int64_t)(kvh * G + head) * hd;
 #pragma unroll
         for (int s = 0; s < HDP; ++s) {
-            const int d = 32 * s + 8 * g;
+            const int d = dim_of(s);
             Raw8<TQ> r = raw8(row + (d < hd ? d : 0));
             if (t < 0 || d >= hd) clear(r);
             to_op(r, qf[rt][s]);
@@ -269,12 +274,21 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     const bool outside = hd < 32 * HDP;                     // some lanes hold dims that the head does not have
     uint32_t k_dims[HDP], v_bytes[NV];                      // what a lane adds for its dims (those outside: the row's start)
 #pragma unroll
-    for (int s = 0; s < HDP; ++s) k_dims[s] = 32 * s + 8 * g < hd ? 32 * s + 8 * g : 0;
+    for (int s = 0; s < HDP; ++s) k_dims[s] = dim_of(s) < hd ? dim_of(s) : 0;
 #pragma unroll
     for (int c = 0; c < NV; ++c) v_bytes[c] = 16 * (4 * c + (lane & 3)) < hd * ES ? 16 * (4 * c + (lane & 3)) : 0;
     const auto load_keys = [&](Block& b, int u, const TC* at, uint32_t off) {
+        if constexpr (PAIRS) {
 #pragma unroll
-        for (int s = 0; s < HDP; ++s) b.kr[u][s] = raw8(at + (off + k_dims[s]));
+            for (int s = 0; s < HDP; s += 2) {
+                const uint4 both = *reinterpret_cast<const uint4*>(at + (off + k_dims[s]));
+                b.kr[u][s].a = make_uint2(both.x, both.y);
+                b.kr[u][s + 1].a = make_uint2(both.z, both.w);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < HDP; ++s) b.kr[u][s] = raw8(at + (off + k_dims[s]));
+        }
     };
     const auto load_values = [&](Block& b, int u, const TC* at, uint32_t off) {
 #pragma unroll
@@ -370,7 +384,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 Op8<TQ> a;
-                if (outside && 32 * s + 8 * g >= hd) clear(b.kr[u][s]);
+                if (outside && dim_of(s) >= hd) clear(b.kr[u][s]);
                 to_op(b.kr[u][s], a);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
