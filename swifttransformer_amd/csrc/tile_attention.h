@@ -11,8 +11,8 @@
 //   O^T += V^T P^T   P^T is the scores' registers as they are.  V goes through LDS, a wave's block in its own part (no barrier), and
 //                    comes back transposed.
 //
-// Keys and values in 8 bits (csrc/small_float.h) become bfloat16 (exact) or float on their way into the product; a key's power of two
-// multiplies its scores, a value's its probability, both without rounding.  Probabilities are rounded to bfloat16 for the second product (at most 2^-8
+// Keys and values in 8 bits (csrc/small_float.h) become bfloat16 (exact) or float on their way into the product; a key's power of two is part of
+// its conversion (float: it multiplies its scores), a value's multiplies its probability, all without rounding.  Probabilities are rounded to bfloat16 for the second product (at most 2^-8
 // of each, as the queries and keys that they come from are), or stay float in the float instances; maxima, sums and normalisers are float.
 #pragma once
 
@@ -39,6 +39,12 @@ template <> struct Raw8<float> { uint4 a, b; };
 template <typename TC> __device__ inline Raw8<TC> raw8(const TC* p) { return *reinterpret_cast<const Raw8<TC>*>(p); }
 template <typename TC> __device__ inline void clear(Raw8<TC>& r) { r = Raw8<TC>{}; }
 
+__device__ inline void flip(Raw8<bf16_t>& r) { r.a.x ^= 0x80008000u; r.a.y ^= 0x80008000u; r.a.z ^= 0x80008000u; r.a.w ^= 0x80008000u; }
+__device__ inline void flip(Raw8<float>& r) {
+    r.a.x ^= 0x80000000u; r.a.y ^= 0x80000000u; r.a.z ^= 0x80000000u; r.a.w ^= 0x80000000u;
+    r.b.x ^= 0x80000000u; r.b.y ^= 0x80000000u; r.b.z ^= 0x80000000u; r.b.w ^= 0x80000000u;
+}
+
 template <typename TQ> struct Op8;
 template <> struct Op8<bf16_t> { bf16x8 v; };
 template <> struct Op8<float> { float v[8]; };
@@ -49,9 +55,9 @@ __device__ inline void to_op(const Raw8<float>& r, Op8<float>& o) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = __uint_as_float(w[i]);
 }
-__device__ inline void to_op(const Raw8<e4m3_t>& r, Op8<bf16_t>& o) {
-    o.v = __builtin_bit_cast(bf16x8, make_uint4(e4m3x2_to_bf16x2<false>(r.a.x, 1.f), e4m3x2_to_bf16x2<true>(r.a.x, 1.f),
-                                                e4m3x2_to_bf16x2<false>(r.a.y, 1.f), e4m3x2_to_bf16x2<true>(r.a.y, 1.f)));
+__device__ inline void to_op(const Raw8<e4m3_t>& r, Op8<bf16_t>& o, float unit = 1.f) {      // times a power of two
+    o.v = __builtin_bit_cast(bf16x8, make_uint4(e4m3x2_to_bf16x2<false>(r.a.x, unit), e4m3x2_to_bf16x2<true>(r.a.x, unit),
+                                                e4m3x2_to_bf16x2<false>(r.a.y, unit), e4m3x2_to_bf16x2<true>(r.a.y, unit)));
 }
 __device__ inline void to_op(const Raw8<e4m3_t>& r, Op8<float>& o) {
     const float2v a = e4m3x2_to_floats<false>(r.a.x), b = e4m3x2_to_floats<true>(r.a.x);
@@ -167,6 +173,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     constexpr int DT = 2 * HDP, R = 16 * RT;
     constexpr bool QUANT = sizeof(TC) == 1;
     constexpr int ES = sizeof(TC);
+    // A key's power of two goes into its conversion to bfloat16 (at no cost, and exact but for what is below 2^-126), into its scores where it becomes float.
+    constexpr bool SCALED = QUANT && sizeof(TQ) == 2;
     using S = Shape<TQ, TC, HDP, RT>;
     constexpr int NU = S::NU, NV = S::NV, KEYS = 16 * NU, NF = NU / 2;
     constexpr int VB = Values<TC, HDP, NU>::kBytes;
@@ -185,6 +193,10 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     // (a dot product takes its dims in any order).
     constexpr bool PAIRS = QUANT && HDP % 2 == 0;
     const auto dim_of = [&](int s) { return PAIRS ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+
+    // Scores in units of log2 are products times sl > 0, so that their maximum is that of the products: the scale's sign goes to the
+    // queries, and with a scale of nothing they are nothing.
+    const float scale = fabsf(p.scale) * 1.44269504088896340736f, sl = scale == 0.f ? 1.f : scale;
 
     // ---- query rows
     Op8<TQ> qf[RT][HDP];
@@ -205,7 +217,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         for (int s = 0; s < HDP; ++s) {
             const int d = dim_of(s);
             Raw8<TQ> r = raw8(row + (d < hd ? d : 0));
-            if (t < 0 || d >= hd) clear(r);
+            if (t < 0 || d >= hd || scale == 0.f) clear(r);
+            if (p.scale < 0.f) flip(r);
             to_op(r, qf[rt][s]);
         }
         if (wave == 0 && g == 0) s_t[16 * rt + r16] = t;     // (read only where the waves share their rows)
@@ -265,8 +278,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     struct Block {
         Raw8<TC> kr[NU][HDP];
         uint4 vr[NU][NV];
-        // exponents of the powers of two: WHOLE, of the four keys and values that a lane has scores of in each 16; else lane l's number f is that of
-        // key 64 f + l, values behind keys
+        // exponents of the powers of two.  WHOLE: of the values of the four keys that a lane has scores of in each 16, and of those four keys or (SCALED) the key
+        // that it loads; else lane l's number f is that of key 64 f + l, values behind keys
         uint32_t field[WHOLE ? 2 * NU : NF];
         uint64_t bad;                                       // keys whose page is none of the pool's
     };
@@ -311,7 +324,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 for (int u = 0; u < NU; ++u) {
                     const uint64_t at = (uint64_t)((uint32_t)q.page[u] < (uint32_t)p.num_pages ? (uint32_t)q.page[u] : 0u) * (uint64_t)p.exp_stride +
                                         (uint64_t)(kvh * ps + (q.row[u] & ~15));
-                    b.field[2 * u] = *reinterpret_cast<const uint32_t*>(p.k_exp + at + 4 * g);
+                    b.field[2 * u] = SCALED ? p.k_exp[at + r16] : *reinterpret_cast<const uint32_t*>(p.k_exp + at + 4 * g);
                     b.field[2 * u + 1] = *reinterpret_cast<const uint32_t*>(p.v_exp + at + 4 * g);
                 }
             }
@@ -342,7 +355,6 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    const float sl = p.scale * 1.44269504088896340736f;     // scores in units of log2
 
     // a block in registers -> maximum, normaliser and sums; `then` is called once its registers are free
     // (What the compiler knows of a product's result and of loads under way ends at a branch: two remain between the products, the mask of a
@@ -374,6 +386,10 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int f = 0; f < NF; ++f) s_unit[64 * f + lane] = __uint_as_float(b.field[f] << 23);
         wave_fence();
+        float k_unit[NU];
+        if constexpr (SCALED)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) k_unit[u] = WHOLE ? __uint_as_float(b.field[2 * u] << 23) : s_unit[16 * u + r16];
         floatx4 sc[RT][NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -384,8 +400,10 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 Op8<TQ> a;
-                if (outside && dim_of(s) >= hd) clear(b.kr[u][s]);
-                to_op(b.kr[u][s], a);
+                // (dims outside: nothing times a dim of the same key, which may be infinite but in 8 bits)
+                if (!QUANT && outside && dim_of(s) >= hd) clear(b.kr[u][s]);
+                if constexpr (SCALED) to_op(b.kr[u][s], a, k_unit[u]);
+                else to_op(b.kr[u][s], a);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
             }
@@ -397,21 +415,20 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int f = 0; f < NF; ++f) vraw[dt][f] = value_raw<HDP>(s_v + 32 * f * Values<TC, HDP, NU>::kPitch, dt, g, r16);
-        floatx4 ku[NU], vu[NU];                             // powers of two, the keys' with the scale
+        floatx4 ku[NU], vu[NU];                             // powers of two
         if (QUANT) {
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 if constexpr (WHOLE) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        ku[u][r] = __uint_as_float(((b.field[2 * u] >> (8 * r)) & 0xffu) << 23);
+                        if (!SCALED) ku[u][r] = __uint_as_float(((b.field[2 * u] >> (8 * r)) & 0xffu) << 23);
                         vu[u][r] = __uint_as_float(((b.field[2 * u + 1] >> (8 * r)) & 0xffu) << 23);
                     }
                 } else {
-                    ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
+                    if (!SCALED) ku[u] = *reinterpret_cast<const floatx4*>(s_unit + 16 * u + 4 * g);
                     vu[u] = *reinterpret_cast<const floatx4*>(s_unit + KEYS + 16 * u + 4 * g);
                 }
-                ku[u] *= sl;
             }
         }
         then();                                             // (the block's registers are free)
@@ -419,7 +436,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int i = 0; i < 4 * NU; ++i) x[rt][i] = sc[rt][i >> 2][i & 3] * (QUANT ? ku[i >> 2][i & 3] : sl);
+            for (int i = 0; i < 4 * NU; ++i) x[rt][i] = QUANT && !SCALED ? sc[rt][i >> 2][i & 3] * ku[i >> 2][i & 3] : sc[rt][i >> 2][i & 3];
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 4 * NU; ++i) {
@@ -438,7 +455,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int i = 2; i < 4 * NU; i += 2) top = max3_raw(top, x[rt][i], x[rt][i + 1]);
             top = rows4_max(top);
-            const float mn = max_raw(m[rt], top);
+            const float mn = max_raw(m[rt], top * sl);
             if (__any(mn > m[rt])) {
                 const float alpha = __builtin_amdgcn_exp2f(m[rt] - mn);
                 l[rt] *= alpha;
@@ -448,7 +465,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
 #pragma unroll
             for (int i = 0; i < 4 * NU; ++i) {
-                x[rt][i] = __builtin_amdgcn_exp2f(x[rt][i] - mn);
+                x[rt][i] = __builtin_amdgcn_exp2f(fmaf(x[rt][i], sl, -mn));
                 l[rt] += x[rt][i];
                 if (QUANT) x[rt][i] *= vu[i >> 2][i & 3];
             }

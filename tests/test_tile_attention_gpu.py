@@ -117,6 +117,20 @@ def test_single_tokens_quant(heads, kv, hd, page, dtype, splits):
     compare(got, torch.stack([w for w, _ in want]), torch.stack([b for _, b in want]))
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 2.0])
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_of_any_size_and_sign(dtype, quant, scale):
+    g = torch.Generator().manual_seed(12)
+    batch = shared_batch([(37, 3)], [1, 40, 77], 4, 2, 80, 16, dtype, quant, g)
+    pool, table, lens, _, _, _, q = batch
+    got = run_shared(batch, 4, scale, shared_splits=2, own_splits=2)
+    for t, n in enumerate(lens):
+        k, v = pool.entries(table, t, n)
+        want, bound = reference(q[t] if scale >= 0 else -q[t], k, v, 4, abs(scale))
+        compare(got[t], want, bound)
+
+
 def test_some_rows_only():
     g = torch.Generator().manual_seed(1)
     table = torch.full((6, 20), -1, dtype=torch.int32)
