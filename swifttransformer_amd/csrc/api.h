@@ -141,11 +141,11 @@ int st_quant_kv_read(void* k_out, void* v_out, const void* k_cache, const void* 
 //                    keys before that, through the block table of the first of them that has a request
 //   else             num_entries rows, row_ids[i] or i, each alone
 // cache_dtype: dtype, or 2 for the 8-bit cache.  Keys in own_splits (and shared_splits) parts; slots is their sum; with more than one,
-// part_o [rows, heads, slots, head_dim] and part_lse [rows, heads, slots] floats (rows: num_rows, or num_entries with row_ids).
+// part_o [rows, heads, slots, head_dim] (sums) and part_ml [rows, heads, slots, 2] (maxima in log2 units, normalisers) floats (rows: num_rows, or num_entries with row_ids).
 struct StTileAttention {
     void* out;
     float* part_o;
-    float* part_lse;
+    float* part_ml;
     const void* q;
     int64_t q_stride;
     const void* k_cache;

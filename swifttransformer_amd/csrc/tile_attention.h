@@ -5,7 +5,7 @@
 // group) pairs: the heads of one token, of the tokens of a prompt's portion, or of all tokens whose requests begin with the same pages.
 // A key is then read once for all of them.  Its four waves take blocks of 32 keys in turn, each with a running maximum, normaliser and
 // sum of its own (an online softmax in float), and meet in LDS at the end; several workgroups that share a row's keys leave
-// normalised sums and log-sum-exps, which a second kernel joins.
+// sums, maxima and normalisers, which a second kernel joins.
 //
 //   S^T = K Q^T      a lane's scores belong to one query row: l % 16.  Keys come from memory as the operand, eight dims a lane.
 //   O^T += V^T P^T   P^T is the scores' registers as they are.  V goes through LDS, a wave's block in its own part (no barrier), and
@@ -525,11 +525,12 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             for (int dt = 0; dt < DT; ++dt) {
                 const int d = 16 * dt + 4 * g;
                 if (16 * dt >= hd) break;
-                const float res[4] = {acc[0][dt][0] * inverse, acc[0][dt][1] * inverse, acc[0][dt][2] * inverse, acc[0][dt][3] * inverse};
+                const float by = p.slots == 1 ? inverse : 1.f;
+                const float res[4] = {acc[0][dt][0] * by, acc[0][dt][1] * by, acc[0][dt][2] * by, acc[0][dt][3] * by};
                 if (p.slots == 1) Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + d, res);
                 else Elem<float>::store4(p.part_o + (at * p.slots + place) * hd + d, res);
             }
-            if (p.slots > 1 && g == 0) p.part_lse[at * p.slots + place] = sum == 0.f ? -INFINITY : m[0] + log2f(sum);
+            if (p.slots > 1 && g == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (at * p.slots + place)) = make_float2(m[0], sum);
         }
         return;
     }
@@ -582,7 +583,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             floatx4 o = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; ++v) o += *reinterpret_cast<const floatx4*>(s_o + (v * R + row) * JP + 4 * quad);
-            const float res[4] = {o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse};
+            const float by = p.slots == 1 ? inverse : 1.f;
+            const float res[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
             if (p.slots == 1)
                 Elem<TQ>::store4((TQ*)p.out + ((int64_t)t * p.heads + head) * hd + d, res);
             else
@@ -591,7 +593,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         if (d0 + DC < DT) __syncthreads();
     }
     if (t >= 0 && p.slots > 1 && quad == 0)
-        p.part_lse[out_row * p.slots + place] = sum == 0.f ? -INFINITY : top + log2f(sum);
+        *reinterpret_cast<float2*>(p.part_ml + 2 * (out_row * p.slots + place)) = make_float2(top, sum);
 }
 
 // LDS of a workgroup
@@ -711,7 +713,8 @@ __global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttenti
     tile_work<TQ, TC, HDP, RT, WHOLE>(p, w, kvh, lds);
 }
 
-// out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s, w_s = 2^(lse_s - max lse): one wave a row and head
+// out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s l_s, w_s = 2^(m_s - max m): one wave a row and head.  (Maxima and normalisers, not the
+// logarithms of their product: those round by 2^-24 of themselves, which at scores of 16 is 2^-20 of a weight.)
 template <typename TQ>
 __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p, int rows) {
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -731,11 +734,10 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p
     const int slots = p.row_start && p.row_start[t] <= 0 ? p.own_splits : p.slots;      // (a row of no group has nothing in the others)
     const int64_t at = (ri * p.heads + head) * p.slots;
     const float* parts = p.part_o + at * hd;
-    const float lse = lane < slots ? p.part_lse[at + lane] : -INFINITY;
-    const float top = wave_max(lse);
-    const float weight = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - top);
-    const uint64_t held = __ballot(lse != -INFINITY);
-    const float sum = wave_sum(weight);
+    const float2 ml = lane < slots ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (at + lane)) : make_float2(kFloor, 0.f);
+    const float weight = __builtin_amdgcn_exp2f(ml.x - wave_max(ml.x));
+    const uint64_t held = __ballot(ml.y != 0.f);            // (parts without a key)
+    const float sum = wave_sum(ml.y * weight);
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
     for (int d = lane; d < hd; d += 64) {
         float o = 0.f;

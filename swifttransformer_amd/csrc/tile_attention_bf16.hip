@@ -29,7 +29,7 @@ extern "C" int st_tile_attention(const StTileAttention* args, hipStream_t stream
     ST_CHECK(p.own_splits >= 1 && (p.num_groups == 0 ? p.shared_splits == 0 : p.shared_splits >= 1) && p.slots == p.own_splits + p.shared_splits && p.slots <= 64,
              "attention: %d and %d splits of the keys in %d places (at most 64)", p.own_splits, p.shared_splits, p.slots);
     if (p.num_rows == 0 || (p.num_entries == 0 && p.num_tiles == 0)) return 0;
-    ST_CHECK(p.out && p.q && (p.slots == 1 || (p.part_o && p.part_lse)), "attention: null operand");
+    ST_CHECK(p.out && p.q && (p.slots == 1 || (p.part_o && p.part_ml)), "attention: null operand");
     ST_CHECK(((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache) |
                reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.part_o)) & 15) == 0 && p.q_stride * (p.dtype == kF32 ? 4 : 2) % 16 == 0,
              "attention: queries, their rows, caches and results must be 16-byte aligned");

@@ -920,7 +920,7 @@ def quant_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Ten
 # ------------------------------------------- attention of rows that read the same keys
 class _TileAttention(ctypes.Structure):
     """Mirror of StTileAttention (csrc/api.h)."""
-    _fields_ = [("out", _c_p), ("part_o", _c_p), ("part_lse", _c_p), ("q", _c_p), ("q_stride", _c_i64), ("k_cache", _c_p), ("v_cache", _c_p),
+    _fields_ = [("out", _c_p), ("part_o", _c_p), ("part_ml", _c_p), ("q", _c_p), ("q_stride", _c_i64), ("k_cache", _c_p), ("v_cache", _c_p),
                 ("page_stride", _c_i64), ("k_exp", _c_p), ("v_exp", _c_p), ("exp_stride", _c_i64), ("token_item", _c_p), ("positions", _c_p),
                 ("block_table", _c_p), ("row_ids", _c_p), ("tile_item", _c_p), ("tile_q0", _c_p), ("item_tok_off", _c_p), ("item_start", _c_p),
                 ("item_len", _c_p), ("row_start", _c_p), ("shared_rows", _c_p), ("group_off", _c_p)] + \
@@ -972,20 +972,20 @@ def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_
     slots = own_splits + shared_splits
     if slots > 64:
         raise KernelError(f"attention: {slots} parts of the keys (at most 64)")
-    part_o = part_lse = 0
+    part_o = part_ml = 0
     if slots > 1:
         n_l = rows * num_q_heads * slots
         if workspace is None:
-            workspace = empty((n_l * (hd + 1),), torch.float32, q.device)
+            workspace = empty((n_l * (hd + 2),), torch.float32, q.device)
         else:
             _need(workspace, "workspace", torch.float32)
             _at(here, workspace, "workspace")
-            if workspace.numel() < n_l * (hd + 1):
+            if workspace.numel() < n_l * (hd + 2):
                 raise KernelError("attention workspace is too small")
         part_o = workspace.data_ptr()
-        part_lse = part_o + 4 * n_l * hd
+        part_ml = part_o + 4 * n_l * hd
     _check(_lib().st_tile_attention(_pack_tiles(
-        out.data_ptr(), part_o, part_lse, q.data_ptr(), row[0] if T > 1 else width, k_cache.data_ptr(), v_cache.data_ptr(), stride,
+        out.data_ptr(), part_o, part_ml, q.data_ptr(), row[0] if T > 1 else width, k_cache.data_ptr(), v_cache.data_ptr(), stride,
         k_exp.data_ptr() if quant else 0, v_exp.data_ptr() if quant else 0, exp_stride, token_item, positions, block_table.data_ptr(), row_ids,
         tile_item, tile_q0, item_tok_off, item_start, item_len, row_start, shared_rows, group_off, T, num_entries, num_tiles, tile_rows, num_shared,
         num_groups, items, pages, ps, num_pages, num_q_heads, nkv, hd, scale, own_splits, shared_splits, slots, code, 2 if quant else code, own_waves, 0), _stream()))
@@ -1017,7 +1017,7 @@ def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     q: [T, num_q_heads*head_dim] view (row stride free), float32 or bfloat16.  Returns [T, num_q_heads*head_dim]; with ``row_ids`` (entries of -1
     are skipped) only those batch rows are computed and written.  A row without an item or a position gets zeros.  ``max_keys``: the most keys that
     a row reads, for the choice of ``num_splits`` where that is 0 (default: what the block table can hold); results do not need it to
-    be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 1)."""
+    be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 2)."""
     here = _here(q, "q")
     T = q.shape[0]
     _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions)
@@ -1076,7 +1076,7 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``row_start`` > 0 has to be in a group.  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
-    ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 1)."""
+    ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 2)."""
     here = _here(q, "q")
     T = q.shape[0]
     if (k_exp is None) != (v_exp is None):

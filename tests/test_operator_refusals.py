@@ -50,7 +50,7 @@ def test_quant_cache():
 def test_tile_attention():
     lib = K._lib()
     p = 4096
-    ok = dict(out=p, part_o=p, part_lse=p, q=p, q_stride=256, k_cache=p, v_cache=p, page_stride=2 * 16 * 64, k_exp=p, v_exp=p, exp_stride=32, token_item=p,
+    ok = dict(out=p, part_o=p, part_ml=p, q=p, q_stride=256, k_cache=p, v_cache=p, page_stride=2 * 16 * 64, k_exp=p, v_exp=p, exp_stride=32, token_item=p,
               positions=p, block_table=p, num_rows=0, num_entries=0, num_items=1, max_pages=4, page_size=16, num_pages=9, heads=4, kv_heads=2, head_dim=64,
               scale=1.0, own_splits=1, slots=1, dtype=1, cache_dtype=2, own_waves=4)
     call = lambda **kw: lib.st_tile_attention(bytes(K._TileAttention(**{**ok, **kw})), None)  # noqa: E731
