@@ -72,6 +72,17 @@ __device__ inline floatx4 mma8(const Op8<float>& a, const Op8<float>& b, floatx4
     for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
     return c;
 }
+// for scores: in float 16 products a chain (one chain over all of a head's dims is two to four times as far off, and an exponent shows it)
+__device__ inline floatx4 scores8(const Op8<bf16_t>& a, const Op8<bf16_t>& b, floatx4 c) { return mma8(a, b, c); }
+__device__ inline floatx4 scores8(const Op8<float>& a, const Op8<float>& b, floatx4 c) {
+    floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], x, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[4 + i], b.v[4 + i], y, 0, 0, 0);
+    }
+    return c + (x + y);
+}
 __device__ inline void weights_to_op(const float* p, Op8<bf16_t>& o) {
     o.v = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])));
 }
@@ -405,7 +416,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                 if constexpr (SCALED) to_op(b.kr[u][s], a, k_unit[u]);
                 else to_op(b.kr[u][s], a);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) sc[rt][u] = mma8(a, qf[rt][s], sc[rt][u]);
+                for (int rt = 0; rt < RT; ++rt) sc[rt][u] = scores8(a, qf[rt][s], sc[rt][u]);
             }
         // (8-bit values: asked for before the softmax that their trip from LDS takes as long as, where registers are left for them)
         constexpr bool EARLY = QUANT && HDP <= 4;
@@ -486,15 +497,16 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         }
     };
     int kb = kb0 + (w.waves == 1 ? 0 : KEYS * wave);
+    constexpr bool AHEAD = WHOLE || HDP <= 4;               // (a lane's own places take registers that the longest heads have not left)
     Places next;
     const auto ahead = [&](Block& b, int at) {              // asks for the block at `at`, whose pages are known, and for the pages of the one behind
-        const Places now = next;                            // (whether or not there is one: what is asked for twice is the last key)
-        next = look_up_block(at + STEP);
+        const Places now = AHEAD ? next : look_up_block(at);       // (whether or not there is one: what is asked for twice is the last key)
+        if (AHEAD) next = look_up_block(at + STEP);
         issue(b, now, at);
     };
     Block one;
     if (kb < ke) {
-        next = look_up_block(kb);
+        if (AHEAD) next = look_up_block(kb);
         ahead(one, kb);
         if constexpr (S::kTwo) {
             Block two;
