@@ -13,8 +13,14 @@
 //            above which little more than k logits lie.  They go to a list in LDS, and what is left to do is done there.
 //   top p    (and a top k above 512) weights (or ones) are summed by 2,048 steps of the value.  The step that holds the border is known
 //            then, and from the steps' weights how many there are up to it; if they are few they go to the list, else the pass that sums
-//            weights for the draw leaves out that step and gathers its keys (value, then index), which are divided in LDS until one is left.  A step with more than 4,096 in it (a row of few values) is divided by passes over the row (cut_order).
+//            weights for the draw leaves out that step and gathers its keys (value, then index), which are divided in LDS until one is
+//            left.  A step with more than 4,096 in it (a row of few values) is divided by passes over the row (cut_order).
 //   draw     in the list; or, where many are kept, by sums over the waves' stretches, over lines of 64 of one, over a line.
+//
+// What bounds it: the passes' instructions, not memory: a weight is 34 of them, most on doubles.  A row of 50,272 alone: 16 us by top k 50 with all
+// other filters, 21 by temperature alone (the largest, weights, draw), 45 by top p of a flat row (weights twice, and the border's keys).  256 rows of
+// 128,007 by top p, flat: 115 us, where reading them once takes 27.  Passes read the row again from the L2: held in registers it was slower, since the
+// unrolled code waits for its own instructions (the largest of 64 rows 35 us, 10 this way).
 #include "api.h"
 #include "common.h"
 

@@ -12,8 +12,17 @@
 //                    comes back transposed.
 //
 // Keys and values in 8 bits (csrc/small_float.h) become bfloat16 (exact) or float on their way into the product; a key's power of two is part of
-// its conversion (float: it multiplies its scores), a value's multiplies its probability, all without rounding.  Probabilities are rounded to bfloat16 for the second product (at most 2^-8
-// of each, as the queries and keys that they come from are), or stay float in the float instances; maxima, sums and normalisers are float.
+// its conversion (float: it multiplies its scores), a value's multiplies its probability, all without rounding.  Probabilities are rounded to
+// bfloat16 for the second product (at most 2^-8 of each, as the queries and keys that they come from are), or stay float in the float
+// instances; maxima, sums and normalisers are float.
+//
+// What bounds it, and what was measured for it (bfloat16 over the 8-bit cache; a large copy reaches 4.9 TB/s, a large product 1,220 TFLOP/s):
+//   single tokens    the cache's bytes: 64 rows of up to 1,000 keys, 8 key heads of 128: 133 MB in 29 us, 4.6 TB/s; 64 of 4,000: 4.6 TB/s.
+//   tiles, prefixes  instructions: a block of 32 keys for 32 rows of 128 dims is 32 matrix instructions (256 cycles) and about 230 others (920), most of
+//                    them conversions and the softmax.  200 rows in groups of 67 behind 6,000 keys: 72 us, of which the SIMDs issue for half.
+//                    So 32 rows a wave (16: 89 us; 64, which leave a wave a SIMD: 97), powers and the scale where they cost nothing (77 -> 72), and two
+//                    products' dims by one load (91 -> 76; the 64 rows above 35 -> 30).
+//   few short rows   the way from the lists to the first key, five dependent reads, and the join: 4 to 5 us of each workgroup.
 #pragma once
 
 #include "api.h"
@@ -129,7 +138,8 @@ __device__ inline void wave_fence() {
 // subtiles of 16 dims that the waves' results are joined by at a time: so many that each thread has a quad of a row's dims
 template <int RT> constexpr int turn_subtiles() { return 4 / RT; }
 
-// Subtiles of 16 keys a block, and whether two blocks are held, one on its way while the other is used (where the registers do for that).
+// Subtiles of 16 keys a block, and whether two blocks are held, one on its way while the other is used: where two waves a SIMD keep their
+// registers.  (Else one, asked for when its registers are free: 40 float rows of 80 dims behind a prefix 39 us with two and a wave a SIMD, 31 with one.)
 template <typename TQ, typename TC, int HDP, int RT> struct Shape {
     static constexpr int NU = 2;
     static constexpr int NV = (2 * HDP * (int)sizeof(TC) + 3) / 4;             // 16-byte chunks of a value that a lane moves (four lanes a value)
@@ -289,8 +299,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     struct Block {
         Raw8<TC> kr[NU][HDP];
         uint4 vr[NU][NV];
-        // exponents of the powers of two.  WHOLE: of the values of the four keys that a lane has scores of in each 16, and of those four keys or (SCALED) the key
-        // that it loads; else lane l's number f is that of key 64 f + l, values behind keys
+        // exponents of the powers of two.  WHOLE: of the values of the four keys that a lane has scores of in each 16, and of those four keys
+        // or (SCALED) the key that it loads; else lane l's number f is that of key 64 f + l, values behind keys
         uint32_t field[WHOLE ? 2 * NU : NF];
         uint64_t bad;                                       // keys whose page is none of the pool's
     };
@@ -793,6 +803,7 @@ template <typename TQ, typename TC, int HDP, int MAX>
 int launch_tiles_of(const StTileAttention& p, hipStream_t stream) {
     const bool whole = p.page_size % 16 == 0 &&
                        (sizeof(TC) > 1 || ((reinterpret_cast<uintptr_t>(p.k_exp) | reinterpret_cast<uintptr_t>(p.v_exp) | (uintptr_t)p.exp_stride) & 3) == 0);
+    // (rows go by MAX subtiles where a group's, or a tile's, fill more than one: 200 rows in three groups 72 us, 89 by one; 512 of a prompt behind 1,024 29, 38 by one)
     const bool many = (int64_t)p.num_shared * (p.heads / p.kv_heads) > 16 * (int64_t)p.num_groups;
     if (p.num_groups > 0) {
         if (!whole) return launch_tiles<TQ, TC, HDP, 1, 1, false>(p, stream);

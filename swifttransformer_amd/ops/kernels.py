@@ -863,7 +863,7 @@ def quant_kv_write(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Te
     k_exp/v_exp: uint8 [num_pages, num_kv_heads, page_size].  A token's head x is stored as e4m3(x * 2^(127 - e)), rounded to nearest even, and e, the
     smallest exponent with which the largest finite magnitude is at most 448 (127 for a head of zeros).  What is not finite becomes NaN.
     k_src/v_src: [T, num_kv_heads*head_dim] views with a common row stride, float32 or bfloat16.  A token without an item or a position, or whose page
-    is none of the pool's, is left out; a (item, position) pair may come once in a call."""
+    is none of the pool's, is left out; no two tokens of a call may have the same place in the cache.  What else the pages hold stays as it is."""
     here = _here(k_cache, "k_cache")
     num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(here, k_cache, v_cache, k_exp, v_exp)
     if ps != page_size:
@@ -939,7 +939,11 @@ def _compute_units(device: int) -> int:
 
 
 def tile_splits(workgroups: int, max_keys: int, units: int) -> int:
-    """Parts that the keys are split into, for ``workgroups`` without a split."""
+    """Parts that the keys are split into, for ``workgroups`` without a split: as many as give each compute unit one, of 256 keys at least.
+
+    More only adds what every workgroup pays, 4 to 5 us from its lists to its first keys and from its sums to their join.  Measured (8-bit cache, bfloat16):
+    one row of 32,000 keys, 32 heads of 64: 165 us whole, 32 in 8 parts (the rule's), 39 in 32; 8 rows of 8,200, 8 key heads of 128: 80, 35 in 4
+    (the rule's), 43 in 16; 64 rows of 4,000: 115 whole (the rule's), 121 in 2."""
     return max(1, min(-(-units // max(1, workgroups)), max_keys // 256, 32))
 
 
@@ -993,9 +997,10 @@ def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_
 
 
 def tile_waves(rows: int, max_keys: int, units: int) -> int:
-    """Waves that share a row's keys: one where there is a wave for every SIMD without sharing, or where there is a block or two
-    of keys for each of four at most."""
-    return 1 if rows >= 4 * units or max_keys <= 128 else 4
+    """Waves that share a row's keys: one where that leaves a wave for every SIMD and a row's keys are few, so that the join of four costs more than it
+    gives.  Measured, one wave and four, 8 key heads of 128, bfloat16 over 8 bits: 256 rows of 100 keys 17 and 24 us, of 600 keys 68 and 63; 200 rows of 300 behind
+    shared prefixes 70 and 74; 16 rows of 100 and a shared prefix (fewer than the SIMDs) 13.7 and 12.9."""
+    return 1 if rows >= 4 * units and max_keys <= 512 else 4
 
 
 def _key_bound(max_keys: int, block_table: torch.Tensor, page_size: int) -> int:
@@ -1029,7 +1034,8 @@ def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if num_splits <= 0:
         num_splits = tile_splits(rows * nkv, bound, units)
     return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, rows, num_splits, 0, out, workspace,
-                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_ids=ids, num_entries=rows, own_waves=tile_waves(rows * nkv * num_splits, bound, units))
+                           token_item=token_item.data_ptr(), positions=positions.data_ptr(), row_ids=ids, num_entries=rows,
+                           own_waves=tile_waves(rows * nkv * num_splits, bound, units))
 
 
 @_timed("attention_prefill_quant", _d_attention_quant)
@@ -1040,7 +1046,8 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_prefill`` over the 8-bit cache: tiles of ``tile_rows`` consecutive query rows of prompt portions.  Tile i covers rows
     [tile_q0[i], tile_q0[i]+tile_rows) of item tile_item[i] (-1: none); row r of an item sits at batch row item_tok_off[item]+r and at position
-    item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
+    item_start[item]+r.  Rows that no tile covers are left as they are.  A value that is not finite reaches
+    its tile's rows, also those before it.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
     ``attention_rows_quant``."""
     here = _here(q, "q")
     nt = tile_item.shape[0]
@@ -1050,8 +1057,8 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise KernelError(f"tiles of {tile_rows} rows")
     nkv = k_cache.shape[1]
     if num_splits <= 0:
-        num_splits = tile_splits(nt * nkv * max(1, tile_rows * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16)), _key_bound(max_keys, block_table, k_cache.shape[2]),
-                                 _compute_units(here))
+        chunks = max(1, tile_rows * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16))
+        num_splits = tile_splits(nt * nkv * chunks, _key_bound(max_keys, block_table, k_cache.shape[2]), _compute_units(here))
     return _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_heads, scale, q.shape[0], num_splits, 0, out, workspace,
                            tile_item=tile_item.data_ptr(), tile_q0=tile_q0.data_ptr(), item_tok_off=item_tok_off.data_ptr(),
                            item_start=item_start.data_ptr(), item_len=item_len.data_ptr(), num_tiles=nt, tile_rows=tile_rows)
@@ -1070,9 +1077,11 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_rows`` for a batch whose requests begin with the same tokens, whose keys and values are read once for all of them.
 
-    Group i are the batch rows shared_rows[group_off[i] .. group_off[i+1]) (int32, a row in one group at most); row t of it reads the keys [0, row_start[t]), up to its
-    position, from the pages that the block table of the group's first row with a request names, and [row_start[t], position] through its own.
-    Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own; a row with
+    Group i are the batch rows shared_rows[group_off[i] .. group_off[i+1]) (int32, a row in one group at most); row t of it reads the keys
+    [0, row_start[t]), up to its position, from the pages that the block table of the group's first row with a request names, and
+    [row_start[t], position] through its own.
+    Rows of a group need not have the same ``row_start`` (a value of the prefix that is not
+    finite reaches the group's rows, also those that end before it).  A row of no group has ``row_start`` 0 and reads all through its own; a row with
     ``row_start`` > 0 has to be in a group.  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
@@ -1089,7 +1098,8 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _all_fit(here, torch.int32, (groups + 1,), group_off=group_off)
     nkv, ps, units = k_cache.shape[1], k_cache.shape[2], _compute_units(here)
     if shared_splits <= 0:
-        shared_splits = tile_splits(max(groups, n * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16)) * nkv, _key_bound(max_shared, block_table, ps), units)
+        entries = max(groups, n * (num_q_heads // nkv) // (32 if q.dtype is torch.bfloat16 else 16))
+        shared_splits = tile_splits(entries * nkv, _key_bound(max_shared, block_table, ps), units)
     own = _key_bound(max_own, block_table, ps)
     if own_splits <= 0:
         own_splits = tile_splits(T * nkv, own, units)

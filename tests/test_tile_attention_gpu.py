@@ -117,6 +117,54 @@ def test_single_tokens_quant(heads, kv, hd, page, dtype, splits):
     compare(got, torch.stack([w for w, _ in want]), torch.stack([b for _, b in want]))
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,hd,page", SHAPES)
+def test_many_short_rows(heads, kv, hd, page, dtype, splits):
+    """So many rows that each is a wave's own: several tokens of the same requests, padding rows between."""
+    g = torch.Generator().manual_seed(heads * hd)
+    lens = [1, 9, 33, 64, 70]
+    table = torch.full((len(lens), -(-max(lens) // page) + 1), -1, dtype=torch.int32)
+    pool = Pool(table.numel() + 2, kv, page, hd, dtype, True, g)
+    for r, n in enumerate(lens):
+        pool.fill(table, r, 0, n)
+    T = -(-4 * torch.cuda.get_device_properties(0).multi_processor_count // (kv * splits)) + 3
+    item = torch.randint(-1, len(lens), (T,), generator=g, dtype=torch.int32)
+    position = torch.tensor([int(torch.randint(0, lens[i], (1,), generator=g)) if i >= 0 else 3 for i in item.tolist()], dtype=torch.int32)
+    q = queries(T, heads, hd, dtype, g)
+    k, v, ke, ve = pool.put()
+    assert K.tile_waves(T * kv * splits, table.shape[1] * page, torch.cuda.get_device_properties(0).multi_processor_count) == 1
+    got = K.attention_rows_quant(q.to(DEV), k, v, ke, ve, item.to(DEV), position.to(DEV), table.to(DEV), heads, hd ** -0.5, num_splits=splits).cpu()
+    for t in list(range(0, T, 7)) + [T - 2, T - 1]:
+        n = int(position[t]) + 1 if item[t] >= 0 else 0
+        want, bound = reference(q[t], *pool.entries(table, int(item[t]), n), heads, hd ** -0.5)
+        compare(got[t], want, bound)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,hd,page", SHAPES)
+def test_many_short_rows_behind_prefixes(heads, kv, hd, page, dtype, quant):
+    g = torch.Generator().manual_seed(heads + 3 * hd)
+    pool, table, lens, start, shared, off, q = shared_batch([(50, 3), (19, 2)], [1, 17, 40], heads, kv, hd, page, dtype, quant, g, alone=(12,))
+    n = len(lens)
+    T = -(-4 * torch.cuda.get_device_properties(0).multi_processor_count // kv) + 3
+    rows = [[t for t in range(T) if t % n == r] for r in range(n)]                 # batch row t is request t % n once more
+    listed, at = [], [0]
+    for i in range(len(off) - 1):
+        listed += [t for r in shared[off[i]:off[i + 1]] for t in rows[r]]
+        at.append(len(listed))
+    item, position = ints([t % n for t in range(T)]), ints([lens[t % n] - 1 for t in range(T)])
+    q = queries(T, heads, hd, dtype, g)
+    k, v, ke, ve = pool.put()
+    put = lambda x: x.to(DEV)  # noqa: E731
+    got = K.attention_shared(put(q), k, v, put(item), put(position), put(table), heads, hd ** -0.5, put(ints([start[t % n] for t in range(T)])), put(ints(listed)),
+                             put(ints(at)), k_exp=ke, v_exp=ve, shared_splits=2, own_splits=1).cpu()
+    for t in list(range(0, T, 11)) + [T - 1]:
+        want, bound = reference(q[t], *pool.entries(table, t % n, lens[t % n]), heads, hd ** -0.5)
+        compare(got[t], want, bound)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 2.0])
 @pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
