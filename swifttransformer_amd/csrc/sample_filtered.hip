@@ -820,6 +820,7 @@ extern "C" int st_sample_filtered(int* out, const float* logits, int64_t row_str
                                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, hipStream_t stream) {
     ST_CHECK(num_rows >= 0 && vocab > 0 && row_stride >= vocab, "sample_filtered: bad sizes rows=%d vocab=%d", num_rows, vocab);
     ST_CHECK(vocab <= 1 << 18, "sample_filtered: %d logits a row (at most %d: sums of weights are 64-bit numbers)", vocab, 1 << 18);
+    ST_CHECK(num_rows < 1 << 22, "sample_filtered: %d rows at once", num_rows);        // (a launch has less than 2^32 threads)
     if (num_rows == 0) return 0;
     ST_CHECK(out && logits && uniforms && temperature, "sample_filtered: null operand");
     sample_filtered_kernel<<<num_rows, 1024, 0, stream>>>(out, logits, row_stride, vocab, uniforms, temperature, top_k, top_p, min_p);

@@ -781,8 +781,10 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     q.shared_entries = RTS > 0 ? (int)((int64_t)p.num_shared * G / (16 * (RTS > 0 ? RTS : 1))) + p.num_groups : 0;
     const int64_t own = p.own_waves == 1 ? (entries * p.own_splits + 3) / 4 : entries * p.own_splits;
     const int64_t groups = (own + (int64_t)q.shared_entries * p.shared_splits) * p.kv_heads;
-    ST_CHECK(entries * p.own_splits < ((int64_t)1 << 31), "attention: too many rows at once");
-    ST_CHECK(groups < ((int64_t)1 << 31), "attention: too many rows at once");
+    const int64_t rows = p.num_tiles > 0 ? (int64_t)p.num_tiles * p.tile_rows : p.num_entries;
+    // (a launch has less than 2^32 threads)
+    ST_CHECK(entries * p.own_splits < ((int64_t)1 << 31) && groups < ((int64_t)1 << 24) && rows < ((int64_t)1 << 31) &&
+             (p.slots == 1 || rows * p.heads <= ((int64_t)1 << 25)), "attention: too many rows at once");
     if (groups == 0) return 0;
     constexpr int lds = lds1 > lds2 ? lds1 : lds2;
     if constexpr (lds > 64 * 1024)
@@ -791,7 +793,6 @@ int launch_tiles(const StTileAttention& p, hipStream_t stream) {
     tile_attention_kernel<TQ, TC, HDP, RT, RTS, WHOLE><<<(unsigned)groups, 256, lds, stream>>>(q);
     ST_LAUNCH_CHECK("tile_attention");
     if (p.slots > 1) {
-        const int64_t rows = p.num_tiles > 0 ? (int64_t)p.num_tiles * p.tile_rows : p.num_entries;
         tile_merge_kernel<TQ><<<(unsigned)((rows * p.heads + 3) / 4), 256, 0, stream>>>(q, (int)rows);
         ST_LAUNCH_CHECK("tile_merge");
     }

@@ -20,7 +20,7 @@ def test_sample_filtered():
     call = lambda **kw: lib.st_sample_filtered(*[{**ok, **kw}[n] for n in ok], None, None, None, None)  # noqa: E731
     assert call() == 0
     for bad, says in ((dict(rows=-1), "bad sizes"), (dict(vocab=0), "bad sizes"), (dict(stride=9), "bad sizes"), (dict(vocab=1 << 19, stride=1 << 19), "logits a row"),
-                      (dict(rows=1, logits=None), "null"), (dict(rows=1, uniforms=None), "null"), (dict(rows=1, temperature=None), "null")):
+                      (dict(rows=1 << 22), "at once"), (dict(rows=1, logits=None), "null"), (dict(rows=1, uniforms=None), "null"), (dict(rows=1, temperature=None), "null")):
         assert says in error(call(**bad))
 
 
@@ -65,7 +65,9 @@ def test_tile_attention():
                       (dict(one, own_splits=2, slots=2, part_o=None), "null"), (dict(one, q=None), "null"), (dict(one, q=4104), "aligned"),
                       (dict(one, q_stride=257), "aligned"), (dict(one, out=None), "null"),
                       (dict(num_tiles=1, tile_rows=64), "tiles need"), (dict(own_waves=2), "waves"), (dict(shared, row_start=None), "lists"), (dict(shared, shared_splits=0, slots=1), "splits"),
-                      (dict(shared, row_ids=p), "lists")):
+                      (dict(shared, row_ids=p), "lists"), (dict(num_rows=1 << 30, num_entries=1 << 30), "at once"),
+                      (dict(num_rows=1 << 24, num_entries=1 << 24, own_splits=2, slots=2, own_waves=1), "at once"),
+                      (dict(num_rows=1, num_tiles=1 << 20, tile_rows=65536, tile_item=p, tile_q0=p, item_tok_off=p, item_start=p, item_len=p), "at once")):
         assert says in error(call(**bad)), bad
 
 
