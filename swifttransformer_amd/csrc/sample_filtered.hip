@@ -95,10 +95,11 @@ struct Row {
     double from, rate;                                // weights are 2^((value - from) rate)
     Powers powers;
     __device__ inline float at(int i) const { return max_raw(p[i], -INFINITY); }      // (a NaN logit is never chosen)
+    __device__ inline double weight_of(float x) const { return powers.weight(((double)x - from) * rate); }       // of a finite one
     __device__ inline double weight_whole(float x) const {      // of one from `low` on (an infinity counts as the largest number, of a row whose rate is 0)
         float y;
         asm("v_min_f32 %0, %1, %2" : "=v"(y) : "v"(3.4028234663852886e38f), "v"(x));      // (without the quieting of NaN that fminf asks for)
-        return powers.weight(((double)y - from) * rate);
+        return weight_of(y);
     }
     __device__ inline uint64_t weight(float x) const { return whole(weight_whole(x)); }
     __device__ inline int step(float x) const { return (int)fminf(x == top ? 0.f : (top - x) * scale, (float)(kBins - 1)); }
@@ -481,15 +482,19 @@ __device__ __forceinline__ void sum_stretches(const Row& row, Shared& s, const C
             double w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w[j] = row.weight_whole(x[j]);
-                if constexpr (decltype(plain)::value) w[j] = x[j] > cut.v ? w[j] : 0.0;
-                else w[j] = within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;
+                if constexpr (decltype(plain)::value) {
+                    w[j] = row.weight_of(max_raw(x[j], cut.v));
+                } else {
+                    w[j] = row.weight_whole(x[j]);
+                    w[j] = within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;
+                }
             }
             sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         });
     };
-    // (nothing but a value to be above: six instructions a logit fewer of 34)
-    if (cut.i < 0 && least == 0.0) add(std::true_type());
+    // (nothing but the value to be above where weights begin, which has none itself and stands for all below it, unless it is so far down that
+    // its power is no number: 23 instructions a logit in the place of 33)
+    if (cut.i < 0 && least == 0.0 && row.rate > 0.0 && ((double)cut.v - row.from) * row.rate > -1000.0) add(std::true_type());
     else add(std::false_type());
     const uint64_t stretch = wave_sum64(whole(sum));
     if (lane == 0) s.stretch[wave] = stretch;
