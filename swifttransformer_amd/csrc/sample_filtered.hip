@@ -18,7 +18,7 @@
 //   draw     in the list; or, where many are kept, by sums over the waves' stretches, over lines of 64 of one, over a line.
 //
 // What bounds it: the passes' instructions, not memory: a weight is 34 of them, most on doubles.  A row of 50,272 alone: 16 us by top k 50 with all
-// other filters, 21 by temperature alone (the largest, weights, draw), 45 by top p of a flat row (weights twice, and the border's keys).  256 rows of
+// other filters, 20 by temperature alone (the largest, weights, draw), 45 by top p of a flat row (weights twice, and the border's keys).  256 rows of
 // 128,007 by top p, flat: 115 us, where reading them once takes 27.  Passes read the row again from the L2: held in registers it was slower, since the
 // unrolled code waits for its own instructions (the largest of 64 rows 35 us, 10 this way).
 #include "api.h"
