@@ -17,7 +17,7 @@
 //            left.  A step with more than 4,096 in it (a row of few values) is divided by passes over the row (cut_order).
 //   draw     in the list; or, where many are kept, by sums over the waves' stretches, over lines of 64 of one, over a line.
 //
-// What bounds it: the passes' instructions, not memory: a weight is 34 of them, most on doubles.  A row of 50,272 alone: 16 us by top k 50 with all
+// What bounds it: the passes' instructions, not memory: a weight and its sum are 23 to 33 of them, most on doubles.  A row of 50,272 alone: 16 us by top k 50 with all
 // other filters, 20 by temperature alone (the largest, weights, draw), 45 by top p of a flat row (weights twice, and the border's keys).  256 rows of
 // 128,007 by top p, flat: 115 us, where reading them once takes 27.  Passes read the row again from the L2: held in registers it was slower, since the
 // unrolled code waits for its own instructions (the largest of 64 rows 35 us, 10 this way).
@@ -286,7 +286,7 @@ __device__ __forceinline__ Cut cut_near(const Row& row, Shared& s, int n, uint64
             low = min(low, s.sorted[16 + w]);
         }
     }
-    for (;;) {
+    for (int round = 0; round < 6; ++round) {         // (each leaves 2^-11 of the 64 bits at most)
         const uint64_t range = high - low;
         const int shift = range < kBins ? 0 : 64 - __builtin_clzll(range) - 11;      // range >> shift < 2,048
         __syncthreads();
@@ -339,7 +339,7 @@ __device__ __forceinline__ void cut_order(const Row& row, Shared& s, Cut& cut, u
         const uint32_t key = ordered(x);
         return first || (key >= low && key <= high);
     };
-    for (;;) {
+    for (int round = 0; round < 8; ++round) {         // (the first by steps, then 2^-11 of a value's 32 bits each)
         __syncthreads();
         for (int b = threadIdx.x; b < kBins; b += 1024) {
             s.weight[b] = 0;
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
     row.rate = best < INFINITY ? 1.4426950408889634 / (double)t : 0.0;
     row.from = best < INFINITY ? (double)best : 0.0;
     row.low = best < INFINITY ? fmaxf(best - kSpan * t, -3.4028234663852886e38f) : best;
-    row.scale = fminf((float)kBins / (kSpan * t), 3.0e38f);
+    row.scale = (float)fmin((double)kBins / ((double)kSpan * (double)t), 3.0e38);      // (not zero but for an infinite temperature)
     const double least = min_share > 0.f ? (double)fminf(min_share, 1.f) * 17592186044416.0 : 0.0;
     // a wave's lanes that ask for it get places one behind the other (the counter's old value and up)
     const auto places = [&](uint32_t* counter, uint64_t all) {
@@ -720,7 +720,9 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
         const int bin = (int)s.bin;
         const uint64_t base = s.before;
         // (all that are kept, and perhaps a few more, are not below `line`, and those of the border's step not above `end`)
-        const float line = below_step(bin), end = bin == 0 ? best : best - (float)bin / row.scale * 0.99999f + fabsf(best) * 1e-6f;
+        // (differences that are no float any more lie in the last step: all of the row is close to it then)
+        const float down = (float)bin / row.scale * 0.99999f;
+        const float line = below_step(bin), end = bin == 0 || !(down < 3.0e38f) ? best : best - down + fabsf(best) * 1e-6f;
         // how many there are up to the border: a step's weight over that of its upper end, too few by a step's width (1.5 %) at most
         const float one = 5.684341886080802e-14f;     // 2^-44
         const float falls = (float)row.rate / row.scale;

@@ -98,6 +98,18 @@ def test_temperatures(temperature):
           floats([0.0, 0.0, 0.1, 0.0] * 3))
 
 
+@pytest.mark.parametrize("temperature", [1e37, 1.2e37, 6e37, 1e38, 3.4e38, math.inf])
+@pytest.mark.parametrize("vocab", [700, 3000, 20000])
+def test_differences_that_no_float_holds(vocab, temperature):
+    """Finite logits further apart than the largest number, at temperatures that give all of them weight."""
+    g = torch.Generator().manual_seed(vocab)
+    n = 24
+    x = 3.3e38 * (2 * torch.rand(n, vocab, generator=g) - 1)
+    x[::3] = torch.where(torch.rand(n // 3, vocab, generator=g) < 0.01, x[::3], -x[::3].abs())
+    k = torch.tensor([0, 0, 600, vocab // 2] * 6).int()
+    check(x, torch.rand(n, generator=g), torch.full((n,), temperature), k, floats([0.2, 0.6, 0.9, 0.99, 1.0 - 2.0 ** -20, 1.0] * 4), floats([0.0, 0.0, 0.0, 0.1] * 6))
+
+
 def test_a_step_that_holds_most_of_the_row():
     """Nearly all logits within one step of the histogram, then within one step of that one, down to values a bit apart."""
     g = torch.Generator().manual_seed(9)
