@@ -902,7 +902,8 @@ def _d_quant_kv_read(k_cache, v_cache, k_exp, v_exp, token_item, positions, bloc
 def quant_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, token_item: torch.Tensor,
                   positions: torch.Tensor, block_table: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that the 8-bit cache holds for tokens (their items and positions, int32 [T]): two tensors
-    [T, num_kv_heads*head_dim] of ``dtype``, exact in float32, and in bfloat16 but for what is below its normal numbers.  Zeros for a token that ``quant_kv_write`` would leave out."""
+    [T, num_kv_heads*head_dim] of ``dtype``, exact in float32, and in bfloat16 but for what is below its normal numbers.  Zeros for a
+    token that ``quant_kv_write`` would leave out."""
     here = _here(k_cache, "k_cache")
     num_pages, nkv, ps, hd, stride, exp_stride = _quant_cache(here, k_cache, v_cache, k_exp, v_exp)
     T = token_item.shape[0]
