@@ -100,22 +100,16 @@ template <> struct Elem<bf16_t> {
     }
 };
 
+// The larger of two and three, NaN where one of them is.  Without the quieting of signalling NaNs that fmaxf asks of the compiler (a second
+// instruction per operand that comes out of a matrix instruction or a lane swap), and by instructions that the compiler knows: it counts
+// the wait states that a reader needs behind a matrix instruction (eight slots behind the 16x16x32 bfloat16 product) for those, not for
+// inline assembly, which could read a result before it is there.
+__device__ inline float max_raw(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ inline float max3_raw(float a, float b, float c) { return max_raw(max_raw(a, b), c); }
+
 // Reductions over the four lanes l%16, l%16+16, l%16+32, l%16+48 of a wavefront (the four
 // 16-lane rows), by the row-swap instructions of gfx950 instead of trips through LDS.
 // Every lane gets the result.
-// max without the quieting of signalling NaNs that fmaxf asks of the compiler (a second
-// instruction per operand that comes out of a matrix instruction or a lane swap)
-__device__ inline float max_raw(float a, float b) {
-    float d;
-    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}
-__device__ inline float max3_raw(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-
 __device__ inline float rows4_max(float x) {
     const uint32_t u = __float_as_uint(x);
     const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);

@@ -36,6 +36,13 @@ constexpr float kSpan = 31.25f;                       // e^-31.25 of the largest
 struct Cut { float v; int i; };
 __device__ inline bool within(const Cut& c, float x, int i) { return (x > c.v) | ((x == c.v) & (i <= c.i)); }     // (no branches)
 
+// the larger, of a number and a NaN the number (one instruction: fmaxf would have the compiler quiet both first)
+__device__ inline float max_of(float a, float b) {
+    float d;
+    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
+    return d;
+}
+
 // bits that order as the values do
 __device__ inline uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
@@ -94,7 +101,7 @@ struct Row {
     float scale;                                      // steps of a histogram in one of the value
     double from, rate;                                // weights are 2^((value - from) rate)
     Powers powers;
-    __device__ inline float at(int i) const { return max_raw(p[i], -INFINITY); }      // (a NaN logit is never chosen)
+    __device__ inline float at(int i) const { return max_of(p[i], -INFINITY); }      // (a NaN logit is never chosen)
     __device__ inline double weight_of(float x) const { return powers.weight(((double)x - from) * rate); }       // of a finite one
     __device__ inline double weight_whole(float x) const {      // of one from `low` on (an infinity counts as the largest number, of a row whose rate is 0)
         float y;
@@ -483,7 +490,7 @@ __device__ __forceinline__ void sum_stretches(const Row& row, Shared& s, const C
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if constexpr (decltype(plain)::value) {
-                    w[j] = row.weight_of(max_raw(x[j], cut.v));
+                    w[j] = row.weight_of(max_of(x[j], cut.v));
                 } else {
                     w[j] = row.weight_whole(x[j]);
                     w[j] = within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;
@@ -566,7 +573,7 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             own_i = x[j] > own ? i + 64 * j : own_i;
-            own = max_raw(own, x[j]);
+            own = max_of(own, x[j]);
         }
     });
     const float mine = wave_max(own);
@@ -578,7 +585,7 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
     if (threadIdx.x == 0) s.n = s.near = 0;
     __syncthreads();
     float best = s.top[0];
-    for (int w = 1; w < 16; ++w) best = max_raw(best, s.top[w]);
+    for (int w = 1; w < 16; ++w) best = max_of(best, s.top[w]);
     if (!(t > 0.f) || k == 1 || !(p > 0.f) || best == -INFINITY) {
         int at = own == best ? own_i : 0x7fffffff;
 #pragma unroll
