@@ -764,7 +764,8 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p
     for (int d = lane; d < hd; d += 64) {
         float o = 0.f;
         for (int s = 0; s < slots; ++s)
-            if ((held >> s) & 1) o += __shfl(weight, s, 64) * parts[(int64_t)s * hd + d];
+            // (read from the lane whether or not it has a dim in this turn: a shuffle gives nothing for lanes that are switched off)
+            if ((held >> s) & 1) o += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), s)) * parts[(int64_t)s * hd + d];
         Elem<TQ>::store((TQ*)p.out + (t * p.heads + head) * hd + d, o * inverse);
     }
 }
