@@ -382,18 +382,19 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     // block that has keys to leave out, and the sums' turn to a new maximum, which most blocks of a long row do without.)
     const auto consume = [&](Block& b, int kb, auto then) {
         const uint64_t none = b.bad;
-        if (none != 0) {                                    // (their values are not to be multiplied, not even by nothing)
+        const bool whole = kb >= w.lo && kb + KEYS <= min(ke, least) && none == 0;
+        if (!whole) {                                       // (values that no row sees are not to be multiplied, not even by nothing)
+            const auto out = [&](int in) { return (kb + in >= ke) | (kb + in < w.lo) | (bool)((none >> in) & 1); };
 #pragma unroll
             for (int u = 0; u < NU; ++u)
-                if ((none >> (16 * u + (lane >> 2))) & 1)
+                if (out(16 * u + (lane >> 2)))
 #pragma unroll
                     for (int c = 0; c < NV; ++c) b.vr[u][c] = make_uint4(0, 0, 0, 0);
             if constexpr (!WHOLE)
 #pragma unroll
                 for (int f = 0; f < NF; ++f)
-                    if ((none >> ((64 * f + lane) % KEYS)) & 1) b.field[f] = 127;
+                    if (out((64 * f + lane) % KEYS)) b.field[f] = 127;
         }
-        const bool whole = kb >= w.lo && kb + KEYS <= min(ke, least) && none == 0;
         wave_fence();                                       // (the block before has been read)
 #pragma unroll
         for (int u = 0; u < NU; ++u)
