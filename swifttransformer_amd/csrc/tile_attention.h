@@ -129,6 +129,22 @@ template <int HDP> __device__ inline void value_op(const char* block, int dt, in
     for (int i = 0; i < 8; ++i) o.v[i] = *reinterpret_cast<const float*>(at + ((i & 3) + 16 * (i >> 2)) * P);
 }
 
+// the bits of a register of values' elements that are infinite or NaN, all of them set
+__device__ inline uint32_t not_finite(uint32_t w, bf16_t) { return ((((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu; }
+__device__ inline uint32_t not_finite(uint32_t w, float) { return (w & 0x7f800000u) == 0x7f800000u ? ~0u : 0u; }
+__device__ inline uint32_t not_finite(uint32_t w, e4m3_t) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
+// four elements from memory as floats
+__device__ inline floatx4 four(const bf16_t* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    return floatx4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+}
+__device__ inline floatx4 four(const float* p) { return *reinterpret_cast<const floatx4*>(p); }
+__device__ inline floatx4 four(const e4m3_t* p) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    const float2v a = e4m3x2_to_floats<false>(w), b = e4m3x2_to_floats<true>(w);
+    return floatx4{a.x, a.y, b.x, b.y};
+}
+
 // what has been written to LDS by the lanes of a wave is read by others of it: LDS takes a wave's accesses in order, the compiler must too
 __device__ inline void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -146,6 +162,14 @@ template <typename TQ, typename TC, int HDP, int RT> struct Shape {
     static constexpr int kBlock = NU * (HDP * (int)sizeof(Raw8<TC>) / 4 + 4 * NV);
     static constexpr bool kTwo = 2 * kBlock + RT * (HDP * (int)sizeof(Op8<TQ>) / 4 + 8 * HDP + 8 * NU) <= 200;
 };
+
+// Waves a SIMD that the registers have to leave room for: two, but where float operands (or, over the storage type, heads of more than 128 dims) fill
+// them; four for the smallest instance with groups, which is a register or two above that if it may be.
+template <typename TQ, typename TC, int HDP, int RTS, bool WHOLE> constexpr int simd_waves() {
+    constexpr bool quant = sizeof(TC) == 1, bf16 = sizeof(TQ) == 2;
+    if (quant && bf16 && HDP == 2 && RTS == 1 && WHOLE) return 4;
+    return HDP <= (quant ? (bf16 ? 8 : 4) : (bf16 ? 4 : 3)) ? 2 : 1;
+}
 
 constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
 
@@ -206,8 +230,10 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     float* s_m = reinterpret_cast<float*>(lds);             // [4][R] the waves' maxima
     float* s_l = s_m + 4 * R;                               // [4][R] and normalisers
     int* s_t = reinterpret_cast<int*>(s_l + 4 * R);         // [R] the rows' tokens
-    float* s_unit = s_l + 5 * R + wave * 2 * KEYS;          // the powers of two of a wave's keys, then values
-    char* s_big = reinterpret_cast<char*>(s_l + 5 * R + (QUANT ? 8 * KEYS : 0));
+    int* s_sees = s_t + R;                                  // [R] and how many keys they see
+    int* s_wild = s_sees + R;                               // [4] whether the waves left out values that are not finite
+    float* s_unit = s_l + 6 * R + 4 + wave * 2 * KEYS;      // the powers of two of a wave's keys, then values
+    char* s_big = reinterpret_cast<char*>(s_l + 6 * R + 4 + (QUANT ? 8 * KEYS : 0));
     char* s_v = s_big + wave * VB;                          // [4][KEYS values], at the end the waves' sums
 
     // The first of the eight dims that a lane has in product s.  In 8 bits two products' dims lie behind each other, so that a load brings both
@@ -242,7 +268,10 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             if (p.scale < 0.f) flip(r);
             to_op(r, qf[rt][s]);
         }
-        if (wave == 0 && g == 0) s_t[16 * rt + r16] = t;     // (read only where the waves share their rows)
+        if (wave == 0 && g == 0) {                          // (read only where the waves share their rows)
+            s_t[16 * rt + r16] = t;
+            s_sees[16 * rt + r16] = sees;
+        }
         most = max(most, sees);
         lim[rt] = t < 0 ? 0x7fffffff : sees;                // (a row that is none takes whatever comes)
         least = min(least, lim[rt]);
@@ -377,19 +406,36 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
 
+    // A value that is not finite is not to reach the rows that do not see its key, not even by a product with nothing: in blocks with keys that some
+    // rows see and some do not (a wave's rows alone have none) such elements are cleared, and given to the rows that see them at the end.
+    bool wild = false;
+
     // a block in registers -> maximum, normaliser and sums; `then` is called once its registers are free
     // (What the compiler knows of a product's result and of loads under way ends at a branch: two remain between the products, the mask of a
     // block that has keys to leave out, and the sums' turn to a new maximum, which most blocks of a long row do without.)
     const auto consume = [&](Block& b, int kb, auto then) {
         const uint64_t none = b.bad;
         const bool whole = kb >= w.lo && kb + KEYS <= min(ke, least) && none == 0;
-        if (!whole) {                                       // (values that no row sees are not to be multiplied, not even by nothing)
+        if (!whole) {
             const auto out = [&](int in) { return (kb + in >= ke) | (kb + in < w.lo) | (bool)((none >> in) & 1); };
+            const uint32_t mixed = least < min(ke, kb + KEYS) ? ~0u : 0u;      // (keys that some rows see and some do not)
+            uint32_t odd = 0;
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
-                if (out(16 * u + (lane >> 2)))
+            for (int u = 0; u < NU; ++u) {
+                const uint32_t none_of = out(16 * u + (lane >> 2)) ? ~0u : 0u;
 #pragma unroll
-                    for (int c = 0; c < NV; ++c) b.vr[u][c] = make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < NV; ++c) {
+                    uint4& v = b.vr[u][c];
+                    const auto clear = [&](uint32_t& x) {
+                        const uint32_t n = not_finite(x, TC{}) & mixed;
+                        odd |= n;
+                        x &= ~(n | none_of);
+                    };
+                    clear(v.x); clear(v.y); clear(v.z); clear(v.w);
+                    asm volatile("" : "+v"(odd));
+                }
+            }
+            wild |= __any(odd != 0);
             if constexpr (!WHOLE)
 #pragma unroll
                 for (int f = 0; f < NF; ++f)
@@ -567,6 +613,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             s_l[wave * R + 16 * rt + r16] = l[rt];
         }
     }
+    if (lane == 0) s_wild[wave] = wild;
     __syncthreads();                                        // (and all blocks of values have been read)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -606,6 +653,17 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             floatx4 o = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; ++v) o += *reinterpret_cast<const floatx4*>(s_o + (v * R + row) * JP + 4 * quad);
+            if (s_wild[0] | s_wild[1] | s_wild[2] | s_wild[3]) {
+                // (they were left out from the first block on in which a row sees less than others)
+                const int seen = min(s_sees[row], ke);
+                for (int key = max(kb0 + max(least - kb0, 0) / KEYS * KEYS, w.lo); key < seen; ++key) {
+                    const int pi = page_of(key), page = bt[pi];
+                    if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
+                    const floatx4 x = four((const TC*)p.v_cache + (int64_t)page * p.page_stride + head_off + (key - pi * ps) * hd + d);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] += fabsf(x[r]) < INFINITY ? 0.f : x[r];
+                }
+            }
             const float by = p.slots == 1 ? inverse : 1.f;
             const float res[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
             if (p.slots == 1)
@@ -624,14 +682,14 @@ template <typename TQ, typename TC, int HDP, int RT>
 constexpr int tile_lds() {
     constexpr int kTurn = 4 * 16 * RT * (16 * turn_subtiles<RT>() + 4) * 4;
     constexpr int NU = Shape<TQ, TC, HDP, RT>::NU;
-    return (9 * 16 * RT + (sizeof(TC) == 1 ? 8 * 16 * NU : 0)) * 4 +
+    return (10 * 16 * RT + 4 + (sizeof(TC) == 1 ? 8 * 16 * NU : 0)) * 4 +
            (4 * Values<TC, HDP, NU>::kBytes > kTurn ? 4 * Values<TC, HDP, NU>::kBytes : kTurn);
 }
 
 // Workgroups: key head fastest (a head's workgroups share its keys and, dealt out in turn, an XCD's L2), then splits, then
 // entries: shared prefixes first (kind 2, RTS subtiles of rows), then single tokens or tiles (RT).
 template <typename TQ, typename TC, int HDP, int RT, int RTS, bool WHOLE>
-__global__ __launch_bounds__(256) void tile_attention_kernel(const StTileAttention p) {
+__global__ __launch_bounds__(256, (simd_waves<TQ, TC, HDP, RTS, WHOLE>())) void tile_attention_kernel(const StTileAttention p) {
     extern __shared__ uint4 dyn[];
     char* lds = reinterpret_cast<char*>(dyn);
     const int G = p.heads / p.kv_heads;

@@ -1047,8 +1047,7 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_prefill`` over the 8-bit cache: tiles of ``tile_rows`` consecutive query rows of prompt portions.  Tile i covers rows
     [tile_q0[i], tile_q0[i]+tile_rows) of item tile_item[i] (-1: none); row r of an item sits at batch row item_tok_off[item]+r and at position
-    item_start[item]+r.  Rows that no tile covers are left as they are.  A value that is not finite reaches
-    its tile's rows, also those before it.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
+    item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
     ``attention_rows_quant``."""
     here = _here(q, "q")
     nt = tile_item.shape[0]
@@ -1081,8 +1080,7 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Group i are the batch rows shared_rows[group_off[i] .. group_off[i+1]) (int32, a row in one group at most); row t of it reads the keys
     [0, row_start[t]), up to its position, from the pages that the block table of the group's first row with a request names, and
     [row_start[t], position] through its own.
-    Rows of a group need not have the same ``row_start`` (a value of the prefix that is not
-    finite reaches the group's rows, also those that end before it).  A row of no group has ``row_start`` 0 and reads all through its own; a row with
+    Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own; a row with
     ``row_start`` > 0 has to be in a group.  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.

@@ -1,5 +1,5 @@
-"""What a row does not read does not reach it, whatever lies there: entries of its own pages before its own keys begin.  And what it does read
-arrives, infinities as infinities."""
+"""What a row does not read does not reach it, whatever lies there: entries of its own pages before its own keys begin, values that only other rows
+of its tile or group see.  And what it does read arrives, infinities as infinities."""
 import math
 
 import pytest
@@ -65,6 +65,52 @@ def compare_with_holes(got, q, k, v, heads, scale):
     assert torch.equal(got[holes].isnan(), what[holes].isnan())
     some = ~what[holes].isnan()
     assert torch.equal(got[holes][some], what[holes][some])
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,hd,page", SHAPES)
+def test_rows_of_a_portion_before_a_value_that_is_no_number(heads, kv, hd, page, dtype, splits):
+    g = torch.Generator().manual_seed(hd)
+    cached, T = 21, 70
+    table = torch.full((1, -(-(cached + T) // page)), -1, dtype=torch.int32)
+    pool = Pool(table.shape[1] + 1, kv, page, hd, dtype, True, g)
+    pool.fill(table, 0, 0, cached + T)
+    for key, head, dim in ((cached + 3, 0, 5), (cached + 18, kv - 1, 11), (cached + 18, kv - 1, hd - 1), (cached + 40, 0, 0), (cached + 69, 0, 8)):
+        pool.v[int(table[0, key // page]), head, key % page, dim] = 0x7f if dim else 0xff
+    q = queries(T, heads, hd, dtype, g)
+    put = lambda x: ints(x).to(DEV)  # noqa: E731
+    got = K.attention_prefill_quant(q.to(DEV), *pool.put(), put([0, 0]), put([0, 64]), put([0]), put([cached]), put([T]), table.to(DEV), heads, hd ** -0.5,
+                                    num_splits=splits)
+    k, v = pool.entries(table, 0, cached + T)
+    for t in range(T):
+        compare_with_holes(got[t], q[t], k[:cached + t + 1], v[:cached + t + 1], heads, hd ** -0.5)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,hd,page", SHAPES)
+def test_rows_of_a_group_that_end_before_a_value_that_is_not_finite(heads, kv, hd, page, dtype, quant):
+    """Rows whose positions lie in the prefix, before and behind values of it that are NaN and infinite; requests that share all of it."""
+    g = torch.Generator().manual_seed(hd)
+    prefix = 75
+    table = torch.full((1, -(-90 // page)), -1, dtype=torch.int32)
+    pool = Pool(table.shape[1] + 1, kv, page, hd, dtype, quant, g)
+    pool.fill(table, 0, 0, 90)
+    for key, dim, bits, value in ((20, 3, 0x7f, math.inf), (37, 3, 0x7f, math.inf), (38, 9, 0xff, -math.inf), (64, 12, 0x7f, math.nan), (64, 3, 0x7f, -math.inf),
+                                  (74, 1, 0x7f, math.inf)):
+        pool.v[int(table[0, key // page]), kv - 1, key % page, dim] = bits if quant else value
+    ends = [1, 19, 20, 21, 36, 37, 38, 39, 60, 64, 65, 74, 75, 76, 90]
+    T = len(ends)
+    q = queries(T, heads, hd, dtype, g)
+    put = lambda x: ints(x).to(DEV)  # noqa: E731
+    on = pool.put()
+    k, v = pool.entries(table, 0, 90)
+    for splits in (1, 2):
+        got = K.attention_shared(q.to(DEV), on[0], on[1], put([0] * T), put([n - 1 for n in ends]), table.to(DEV), heads, hd ** -0.5, put([prefix] * T),
+                                 put(range(T)), put([0, T]), k_exp=on[2], v_exp=on[3], shared_splits=splits, own_splits=1)
+        for t, n in enumerate(ends):
+            compare_with_holes(got[t], q[t], k[:n], v[:n], heads, hd ** -0.5)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
