@@ -91,7 +91,7 @@ struct Powers {
         return (__longlong_as_double((long long)((uint64_t)high << 32 | (uint32_t)bits)) + kRound) - kRound;
     }
 };
-// a whole number below 2^52 that a double holds
+// a whole number below 2^52 that a double holds (a weight; sums of 256 may be 2^52)
 __device__ inline uint64_t whole(double w) { return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; }
 
 struct Row {
@@ -503,7 +503,7 @@ __device__ __forceinline__ void sum_stretches(const Row& row, Shared& s, const C
     // its power is no number: 23 instructions a logit in the place of 33)
     if (cut.i < 0 && least == 0.0 && row.rate > 0.0 && ((double)cut.v - row.from) * row.rate > -1000.0) add(std::true_type());
     else add(std::false_type());
-    const uint64_t stretch = wave_sum64(whole(sum));
+    const uint64_t stretch = wave_sum64((uint64_t)sum);
     if (lane == 0) s.stretch[wave] = stretch;
     __syncthreads();
 }
@@ -582,7 +582,11 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
         s.weight[b] = 0;
         s.count[b] = 0;
     }
-    if (threadIdx.x == 0) s.n = s.near = 0;
+    if (threadIdx.x == 0) {
+        s.n = s.near = s.bin = 0;                         // (a place is always found; were one not, no index would be whatever lay here)
+        s.before = 0;
+        s.cut = Cut{0.f, 0};
+    }
     __syncthreads();
     float best = s.top[0];
     for (int w = 1; w < 16; ++w) best = max_of(best, s.top[w]);
@@ -796,7 +800,7 @@ __global__ __launch_bounds__(1024) void sample_filtered_kernel(int* __restrict__
         };
         if (cut.i < 0 && least == 0.0) gather(std::true_type());
         else gather(std::false_type());
-        const uint64_t stretch = wave_sum64(whole(sum));
+        const uint64_t stretch = wave_sum64((uint64_t)sum);
         if (lane == 0) s.stretch[wave] = stretch;
         __syncthreads();
         if (s.near <= kNear) {
