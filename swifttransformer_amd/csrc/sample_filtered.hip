@@ -36,12 +36,8 @@ constexpr float kSpan = 31.25f;                       // e^-31.25 of the largest
 struct Cut { float v; int i; };
 __device__ inline bool within(const Cut& c, float x, int i) { return (x > c.v) | ((x == c.v) & (i <= c.i)); }     // (no branches)
 
-// the larger, of a number and a NaN the number (one instruction: fmaxf would have the compiler quiet both first)
-__device__ inline float max_of(float a, float b) {
-    float d;
-    asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}
+// the larger, of a number and any NaN the number (the hardware's maximum makes a NaN of a signalling one, fmaxf has the compiler quiet both first)
+__device__ inline float max_of(float a, float x) { return x > a ? x : a; }
 
 // bits that order as the values do
 __device__ inline uint32_t ordered(float x) {
@@ -101,7 +97,7 @@ struct Row {
     float scale;                                      // steps of a histogram in one of the value
     double from, rate;                                // weights are 2^((value - from) rate)
     Powers powers;
-    __device__ inline float at(int i) const { return max_of(p[i], -INFINITY); }      // (a NaN logit is never chosen)
+    __device__ inline float at(int i) const { return p[i]; }      // (a NaN is within no cut)
     __device__ inline double weight_of(float x) const { return powers.weight(((double)x - from) * rate); }       // of a finite one
     __device__ inline double weight_whole(float x) const {      // of one from `low` on (an infinity counts as the largest number, of a row whose rate is 0)
         float y;
@@ -490,7 +486,7 @@ __device__ __forceinline__ void sum_stretches(const Row& row, Shared& s, const C
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if constexpr (decltype(plain)::value) {
-                    w[j] = row.weight_of(max_of(x[j], cut.v));
+                    w[j] = row.weight_of(max_of(cut.v, x[j]));
                 } else {
                     w[j] = row.weight_whole(x[j]);
                     w[j] = within(cut, x[j], i + 64 * j) & (w[j] >= least) ? w[j] : 0.0;

@@ -1,10 +1,12 @@
-"""Filtered sampling where most of a row weighs the same as its largest, up to rows of 2^18 logits whose sums of weights are the largest that there are."""
+"""Filtered sampling where most of a row weighs the same as its largest, up to rows of 2^18 logits whose sums of weights are the largest that there are,
+and logits that are signalling NaN."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from test_sample_filtered_gpu import check, floats
+from test_sample_filtered_gpu import check, floats, settings
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +40,16 @@ def test_stretches_of_largest_and_of_smaller(vocab):
     x[:, vocab * 5 // 8:] = -0.5
     x[1::2] = x[1::2].flip(1)
     check(x, u, t, k, p, least)
+
+
+@pytest.mark.parametrize("bits", [0x7f800001, 0x7fa00000, 0x7fbfffff, -0x7fffff, -0x600000])
+@pytest.mark.parametrize("vocab", [3, 700, 5003])
+def test_signalling_nan(vocab, bits):
+    g = torch.Generator().manual_seed(vocab)
+    rows = 24
+    x = 3 * torch.randn(rows, vocab, generator=g)
+    at = torch.rand(rows, vocab, generator=g) < 0.3
+    x.view(torch.int32)[at] = bits
+    x.view(torch.int32)[0] = bits
+    assert bool(np.isnan(x.numpy()[0]).all())
+    check(x, *settings(rows, vocab, g))
