@@ -812,10 +812,33 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p
         t = p.row_ids[ri];
     }
     if (t < 0 || t >= p.num_rows) return;
-    const int slots = p.row_start && p.row_start[t] <= 0 ? p.own_splits : p.slots;      // (a row of no group has nothing in the others)
     const int64_t at = (ri * p.heads + head) * p.slots;
     const float* parts = p.part_o + at * hd;
-    const float2 ml = lane < slots ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (at + lane)) : make_float2(kFloor, 0.f);
+    float2 ml = lane < p.slots ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (at + lane)) : make_float2(kFloor, 0.f);
+    int slots = p.slots;
+    if (p.row_start) {
+        // Nothing has written the prefix's parts of a row that no group lists, or that has no prefix.  (Its place in the lists is looked for in 256 places at a time,
+        // the first of them asked for with all the rest: a row's own loads are one trip to memory.)
+        const int n = p.num_shared, begin = p.group_off[0], end = p.group_off[p.num_groups], start = p.row_start[t];
+        int there[4];
+        const auto ask = [&](int base) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) there[k] = p.shared_rows[min(base + 64 * k + lane, n - 1)];
+        };
+        ask(0);
+        bool listed = false;
+        for (int base = 0;; ask(base)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int place = base + 64 * k + lane;
+                listed |= there[k] == t && place >= begin && place < min(end, n);
+            }
+            listed = __any(listed);
+            if (listed || start <= 0 || (base += 256) >= n) break;
+        }
+        if (!listed || start <= 0) slots = p.own_splits;
+        if (lane >= slots) ml = make_float2(kFloor, 0.f);
+    }
     const float weight = __builtin_amdgcn_exp2f(ml.x - wave_max(ml.x));
     const uint64_t held = __ballot(ml.y != 0.f);            // (parts without a key)
     const float sum = wave_sum(ml.y * weight);

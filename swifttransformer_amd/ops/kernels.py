@@ -1080,8 +1080,8 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Group i are the batch rows shared_rows[group_off[i] .. group_off[i+1]) (int32, a row in one group at most); row t of it reads the keys
     [0, row_start[t]), up to its position, from the pages that the block table of the group's first row with a request names, and
     [row_start[t], position] through its own.
-    Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own; a row with
-    ``row_start`` > 0 has to be in a group.  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
+    Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own (with
+    another one it reads its keys from there on, nothing of a prefix).  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
     ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 2)."""

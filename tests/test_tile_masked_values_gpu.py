@@ -133,3 +133,25 @@ def test_a_last_value_that_is_infinite(dtype, waves):
                                  put(range(T)), put([0, T]), shared_splits=1, own_splits=1)
         compare_with_holes(got[0], q[0], k, v, heads, 0.125)
         compare_with_holes(got[T - 1], q[0], k, v, heads, 0.125)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_rows_with_a_prefix_that_no_group_lists(quant):
+    """They read their own keys from where these begin, and nothing that the workspace held before."""
+    g = torch.Generator().manual_seed(6)
+    batch = shared_batch([(70, 4), (33, 3)], [20, 5], 4, 2, 64, 16, torch.float32, quant, g)
+    pool, table, lens, start, shared, off, q = batch
+    left_out = [shared[1], shared[6]]
+    listed = [-1 if r in left_out else r for r in shared]
+    k, v, ke, ve = pool.put()
+    put = lambda x: ints(x).to(DEV)  # noqa: E731
+    n = len(lens)
+    for rows, at in ((listed, off), (listed + [left_out[0]], off), ([left_out[1]] + listed, [1 + o for o in off]), (listed + [-1] * 300, [0, 4, 307])):
+        # (lists that go on behind the last group, or begin before the first one, and a long one)
+        workspace = torch.full((n * 4 * 4 * 66,), math.nan, device=DEV)
+        got = K.attention_shared(q.to(DEV), k, v, put(range(n)), put([m - 1 for m in lens]), table.to(DEV), 4, 0.125, put(start), put(rows), put(at), k_exp=ke,
+                                 v_exp=ve, shared_splits=2, own_splits=2, workspace=workspace)
+        for t in range(n):
+            kk, vv = pool.entries(table, t, lens[t])
+            first = start[t] if t in left_out else 0
+            compare(got[t], *reference(q[t], kk[first:], vv[first:], 4, 0.125))
