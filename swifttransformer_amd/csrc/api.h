@@ -141,7 +141,7 @@ int st_quant_kv_read(void* k_out, void* v_out, const void* k_cache, const void* 
 //                    keys before that, through the block table of the first of them that has a request
 //   else             num_entries rows, row_ids[i] or i, each alone
 // cache_dtype: dtype, or 2 for the 8-bit cache.  Keys in own_splits (and shared_splits) parts; slots is their sum; with more than one,
-// part_o [rows, heads, slots, head_dim] (sums) and part_ml [rows, heads, slots, 2] (maxima in log2 units, normalisers) floats (rows: num_rows, or num_entries with row_ids).
+// part_o [rows, heads, slots, head_dim] (sums) and part_ml [rows, heads, slots, 2] (maxima of products, normalisers) floats (rows: num_rows, or num_entries with row_ids).
 struct StTileAttention {
     void* out;
     float* part_o;

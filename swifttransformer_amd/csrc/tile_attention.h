@@ -171,7 +171,17 @@ template <typename TQ, typename TC, int HDP, int RTS, bool WHOLE> constexpr int 
     return HDP <= (quant ? (bf16 ? 8 : 4) : (bf16 ? 4 : 3)) ? 2 : 1;
 }
 
-constexpr float kFloor = -1.0e30f;      // a running maximum before the first key
+constexpr float kFloor = -3.4028234663852886e38f;      // a running maximum before the first key
+
+// Scores in units of log2 are products times sl > 0, so that their maximum is that of the products: the scale's sign goes to the queries, and with a
+// scale of nothing they are nothing.
+__device__ inline float log2_scale(float scale) {
+    const float s = fabsf(scale) * 1.44269504088896340736f;
+    return s == 0.f ? 1.f : s;
+}
+// Maxima are those of products, and what is scaled is a difference of two: 2^24 in units of log2 and more, a rounded maximum in those units would be off by
+// more than the weights' range (scores of 10^9 and more came out as nothing or NaN; one instruction a score, 1 % of a portion's time).
+__device__ inline float weight_of(float score, float top, float sl) { return __builtin_amdgcn_exp2f((score - top) * sl); }
 
 // What a workgroup works on: rows [first, first + count) of the flat list (token j, query head) = (f / group, f % group).
 struct TileWork {
@@ -241,9 +251,8 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     constexpr bool PAIRS = QUANT && HDP % 2 == 0;
     const auto dim_of = [&](int s) { return PAIRS ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
 
-    // Scores in units of log2 are products times sl > 0, so that their maximum is that of the products: the scale's sign goes to the
-    // queries, and with a scale of nothing they are nothing.
-    const float scale = fabsf(p.scale) * 1.44269504088896340736f, sl = scale == 0.f ? 1.f : scale;
+    const float sl = log2_scale(p.scale);
+    const bool no_scale = fabsf(p.scale) * 1.44269504088896340736f == 0.f;
 
     // ---- query rows
     Op8<TQ> qf[RT][HDP];
@@ -264,7 +273,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         for (int s = 0; s < HDP; ++s) {
             const int d = dim_of(s);
             Raw8<TQ> r = raw8(row + (d < hd ? d : 0));
-            if (t < 0 || d >= hd || scale == 0.f) clear(r);
+            if (t < 0 || d >= hd || no_scale) clear(r);
             if (p.scale < 0.f) flip(r);
             to_op(r, qf[rt][s]);
         }
@@ -523,9 +532,9 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
             for (int i = 2; i < 4 * NU; i += 2) top = max3_raw(top, x[rt][i], x[rt][i + 1]);
             top = rows4_max(top);
-            const float mn = max_raw(m[rt], top * sl);
+            const float mn = max_raw(m[rt], top);
             if (__any(mn > m[rt])) {
-                const float alpha = __builtin_amdgcn_exp2f(m[rt] - mn);
+                const float alpha = weight_of(m[rt], mn, sl);
                 l[rt] *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
@@ -533,7 +542,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             }
 #pragma unroll
             for (int i = 0; i < 4 * NU; ++i) {
-                x[rt][i] = __builtin_amdgcn_exp2f(fmaf(x[rt][i], sl, -mn));
+                x[rt][i] = weight_of(x[rt][i], mn, sl);
                 l[rt] += x[rt][i];
                 if (QUANT) x[rt][i] *= vu[i >> 2][i & 3];
             }
@@ -620,7 +629,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
         float top = kFloor;
 #pragma unroll
         for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + 16 * rt + r16]);
-        const float own = __builtin_amdgcn_exp2f(m[rt] - top);
+        const float own = weight_of(m[rt], top, sl);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= own;
     }
@@ -634,7 +643,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
 #pragma unroll
     for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + row]);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * __builtin_amdgcn_exp2f(s_m[v * R + row] - top);
+    for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * weight_of(s_m[v * R + row], top, sl);
     // (a sum that is no number belongs to the result)
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t out_row = (int64_t)(w.slot >= 0 ? w.slot : t) * p.heads + head;
@@ -794,7 +803,7 @@ __global__ __launch_bounds__(256, (simd_waves<TQ, TC, HDP, RTS, WHOLE>())) void 
     tile_work<TQ, TC, HDP, RT, WHOLE>(p, w, kvh, lds);
 }
 
-// out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s l_s, w_s = 2^(m_s - max m): one wave a row and head.  (Maxima and normalisers, not the
+// out[row, :] = sum_s w_s part_o[row, s, :] / sum_s w_s l_s, w_s = e^(m_s - max m): one wave a row and head.  (Maxima and normalisers, not the
 // logarithms of their product: those round by 2^-24 of themselves, which at scores of 16 is 2^-20 of a weight.)
 template <typename TQ>
 __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p, int rows) {
@@ -839,7 +848,7 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(const StTileAttention p
         if (!listed || start <= 0) slots = p.own_splits;
         if (lane >= slots) ml = make_float2(kFloor, 0.f);
     }
-    const float weight = __builtin_amdgcn_exp2f(ml.x - wave_max(ml.x));
+    const float weight = weight_of(ml.x, wave_max(ml.x), log2_scale(p.scale));
     const uint64_t held = __ballot(ml.y != 0.f);            // (parts without a key)
     const float sum = wave_sum(ml.y * weight);
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
