@@ -18,10 +18,11 @@
 //
 // What bounds it, and what was measured for it (bfloat16 over the 8-bit cache; a large copy reaches 4.9 TB/s, a large product 1,220 TFLOP/s):
 //   single tokens    the cache's bytes: 64 rows of up to 1,000 keys, 8 key heads of 128: 133 MB in 29 us, 4.6 TB/s; 64 of 4,000: 4.6 TB/s.
-//   tiles, prefixes  instructions: a block of 32 keys for 32 rows of 128 dims is 32 matrix instructions (256 cycles) and about 230 others (920), most of
-//                    them conversions and the softmax.  200 rows in groups of 67 behind 6,000 keys: 72 us, of which the SIMDs issue for half.
-//                    So 32 rows a wave (16: 89 us; 64, which leave a wave a SIMD: 97), powers and the scale where they cost nothing (77 -> 72), and two
-//                    products' dims by one load (91 -> 76; the 64 rows above 35 -> 30).
+//   tiles, prefixes  instructions: a block of 32 keys for 32 rows of 128 dims is 32 matrix instructions (16 cycles each, 512) and about 355 others (four each,
+//                    1,420), most of them conversions and the softmax (counted over a portion of 512 rows: 0.66 and 7.4 million).  200 rows in
+//                    groups of 67 behind 6,000 keys: 70 to 76 us, of which the SIMDs issue for half.  So 32 rows a wave (16: 98 us; 64, which leave a
+//                    wave a SIMD: 97 where 32 took 72), powers of two in conversions (77 -> 72 with the scale in the exponent's product, which
+//                    scores of any size have undone, 1 %), and two products' dims by one load (91 -> 76; the 64 rows above 35 -> 30).
 //   few short rows   the way from the lists to the first key, five dependent reads, and the join: 4 to 5 us of each workgroup.
 #pragma once
 
@@ -896,7 +897,7 @@ template <typename TQ, typename TC, int HDP, int MAX>
 int launch_tiles_of(const StTileAttention& p, hipStream_t stream) {
     const bool whole = p.page_size % 16 == 0 &&
                        (sizeof(TC) > 1 || ((reinterpret_cast<uintptr_t>(p.k_exp) | reinterpret_cast<uintptr_t>(p.v_exp) | (uintptr_t)p.exp_stride) & 3) == 0);
-    // (rows go by MAX subtiles where a group's, or a tile's, fill more than one: 200 rows in three groups 72 us, 89 by one; 512 of a prompt behind 1,024 29, 38 by one)
+    // (rows go by MAX subtiles where a group's, or a tile's, fill more than one: 200 rows in three groups 76 us, 98 by one; 512 of a prompt behind 1,024 31, 39 by one)
     const bool many = (int64_t)p.num_shared * (p.heads / p.kv_heads) > 16 * (int64_t)p.num_groups;
     if (p.num_groups > 0) {
         if (!whole) return launch_tiles<TQ, TC, HDP, 1, 1, false>(p, stream);

@@ -943,8 +943,8 @@ def tile_splits(workgroups: int, max_keys: int, units: int) -> int:
     """Parts that the keys are split into, for ``workgroups`` without a split: as many as give each compute unit one, of 256 keys at least.
 
     More only adds what every workgroup pays, 4 to 5 us from its lists to its first keys and from its sums to their join.  Measured (8-bit cache, bfloat16):
-    one row of 32,000 keys, 32 heads of 64: 165 us whole, 32 in 8 parts (the rule's), 39 in 32; 8 rows of 8,200, 8 key heads of 128: 80, 35 in 4
-    (the rule's), 43 in 16; 64 rows of 4,000: 115 whole (the rule's), 121 in 2."""
+    one row of 32,000 keys, 32 heads of 64: 167 us whole, 32 in 8 parts (the rule's), 40 in 32; 8 rows of 8,200, 8 key heads of 128: 80, 34 in 4
+    (the rule's), 42 in 16; 64 rows of 4,000: 115 whole (the rule's), 112 to 119 in 2 to 8."""
     return max(1, min(-(-units // max(1, workgroups)), max_keys // 256, 32))
 
 
@@ -999,8 +999,8 @@ def _tile_attention(here, q, k_cache, v_cache, k_exp, v_exp, block_table, num_q_
 
 def tile_waves(rows: int, max_keys: int, units: int) -> int:
     """Waves that share a row's keys: one where that leaves a wave for every SIMD and a row's keys are few, so that the join of four costs more than it
-    gives.  Measured, one wave and four, 8 key heads of 128, bfloat16 over 8 bits: 256 rows of 100 keys 17 and 24 us, of 600 keys 68 and 63; 200 rows of 300 behind
-    shared prefixes 70 and 74; 16 rows of 100 and a shared prefix (fewer than the SIMDs) 13.7 and 12.9."""
+    gives.  Measured, one wave and four, 8 key heads of 128, bfloat16 over 8 bits: 256 rows of 100 keys 17 and 26 us, of 600 keys 68 and 64; 200 rows of 300 behind
+    shared prefixes 70 and 75; 16 rows of 100 and a shared prefix (fewer than the SIMDs) 14.3 and 13.5."""
     return 1 if rows >= 4 * units and max_keys <= 512 else 4
 
 
@@ -1023,7 +1023,10 @@ def attention_rows_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     q: [T, num_q_heads*head_dim] view (row stride free), float32 or bfloat16.  Returns [T, num_q_heads*head_dim]; with ``row_ids`` (entries of -1
     are skipped) only those batch rows are computed and written.  A row without an item or a position gets zeros.  ``max_keys``: the most keys that
     a row reads, for the choice of ``num_splits`` where that is 0 (default: what the block table can hold); results do not need it to
-    be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 2)."""
+    be right.  ``workspace``: floats for rows * heads * splits * (head_dim + 2).
+
+    With bfloat16 queries probabilities are rounded to bfloat16 (2^-8 of each at most) for their product with the values, where
+    ``attention_rows`` keeps them in float: results are 3 to 8 % further from 64-bit arithmetic than a last rounding alone."""
     here = _here(q, "q")
     T = q.shape[0]
     _all_fit(here, torch.int32, (T,), token_item=token_item, positions=positions)
@@ -1047,8 +1050,8 @@ def attention_prefill_quant(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_prefill`` over the 8-bit cache: tiles of ``tile_rows`` consecutive query rows of prompt portions.  Tile i covers rows
     [tile_q0[i], tile_q0[i]+tile_rows) of item tile_item[i] (-1: none); row r of an item sits at batch row item_tok_off[item]+r and at position
-    item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q) as in
-    ``attention_rows_quant``."""
+    item_start[item]+r.  Rows that no tile covers are left as they are.  ``max_keys``, ``num_splits``, ``workspace`` (for all rows of q), and the
+    probabilities' rounding, as in ``attention_rows_quant``."""
     here = _here(q, "q")
     nt = tile_item.shape[0]
     _all_fit(here, torch.int32, (nt,), tile_item=tile_item, tile_q0=tile_q0)
@@ -1081,7 +1084,9 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     [0, row_start[t]), up to its position, from the pages that the block table of the group's first row with a request names, and
     [row_start[t], position] through its own.
     Rows of a group need not have the same ``row_start``.  A row of no group has ``row_start`` 0 and reads all through its own (with
-    another one it reads its keys from there on, nothing of a prefix).  With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type.
+    another one it reads its keys from there on, nothing of a prefix).
+    With ``k_exp`` and ``v_exp`` the cache is the 8-bit one (``quant_kv_write``), else of q's type; with bfloat16 queries probabilities are rounded
+    as in ``attention_rows_quant``, over either, which ``attention_rows`` does not do.
     All lists live on the device, so a recorded call serves any groups of its sizes.  ``max_shared``, ``max_own``: the most keys of both kinds that a
     row reads, for the choice of the splits that are 0 (default: what the block table can hold); results do not need them to be right.
     ``workspace``: floats for T * heads * (shared + own splits) * (head_dim + 2)."""

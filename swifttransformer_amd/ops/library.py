@@ -35,7 +35,9 @@ HIPCC_FLAGS = [
 ]
 # per-file additions: the prompt attention kernels keep their matrix-core accumulators in ordinary
 # vector registers, where the softmax rescales them without moves to and from the
-# accumulation registers
+# accumulation registers.  The tile_attention files for their results too: without it heads of 256 came out wrong, a product's result
+# read right behind a branch, while the scores' maxima still were inline assembly, for which no wait states are counted; they have not been
+# built without it since
 FILE_FLAGS = {"attention_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_prefill_dma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_prefill_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
