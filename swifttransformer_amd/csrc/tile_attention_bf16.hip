@@ -22,7 +22,8 @@ extern "C" int st_tile_attention(const StTileAttention* args, hipStream_t stream
              "attention: page stride %lld is smaller than a page, unaligned or too large", (long long)p.page_stride);
     ST_CHECK(p.cache_dtype != 2 || (p.k_exp && p.v_exp && p.exp_stride >= (int64_t)p.kv_heads * p.page_size), "attention: an 8-bit cache needs its exponents");
     ST_CHECK(p.cache_dtype == 2 || p.num_groups > 0, "attention: single tokens and tiles over a cache of the queries' type have kernels of their own");
-    ST_CHECK(p.num_groups == 0 || (p.row_start && p.shared_rows && p.group_off && p.num_tiles == 0 && !p.row_ids), "attention: shared prefixes need their lists");
+    ST_CHECK(p.num_groups == 0 ? !p.row_start : p.row_start && p.shared_rows && p.num_shared > 0 && p.group_off && p.num_tiles == 0 && !p.row_ids,
+             "attention: shared prefixes need their lists, and rows that start behind one need the prefixes");
     ST_CHECK(p.num_tiles == 0 || (p.tile_rows > 0 && p.tile_rows <= 65536 && p.tile_item && p.tile_q0 && p.item_tok_off && p.item_start && p.item_len),
              "attention: tiles need their lists");
     ST_CHECK(p.own_waves == 4 || (p.own_waves == 1 && p.num_tiles == 0), "attention: %d waves a row (4, or 1 without tiles)", p.own_waves);
