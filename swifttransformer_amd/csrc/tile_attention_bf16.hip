@@ -14,7 +14,8 @@ extern "C" int st_tile_attention(const StTileAttention* args, hipStream_t stream
              p.page_size > 0 && p.max_pages > 0 && p.num_pages > 0 && p.num_items > 0, "attention: bad sizes");
     ST_CHECK(p.heads % p.kv_heads == 0, "attention: %d query heads do not divide into %d key heads", p.heads, p.kv_heads);
     ST_CHECK(p.head_dim > 0 && p.head_dim % 16 == 0 && p.head_dim <= 256, "attention: head_dim %d is no multiple of 16 up to 256", p.head_dim);
-    ST_CHECK((int64_t)p.max_pages * p.page_size < 0x7fffffff, "attention: a block table of more than 2^31 positions");
+    // (keys are counted by ints, up to two rounds of the waves' blocks, 128 keys each, past the last one)
+    ST_CHECK((int64_t)p.max_pages * p.page_size <= 0x7fffffff - 512, "attention: a block table of close to 2^31 positions or more");
     ST_CHECK(p.dtype == kF32 || p.dtype == kBF16, "attention: unknown dtype %d", p.dtype);
     ST_CHECK(p.cache_dtype == p.dtype || p.cache_dtype == 2, "attention: a cache of type %d under queries of type %d", p.cache_dtype, p.dtype);
     const int elem = p.cache_dtype == 2 ? 1 : p.dtype == kF32 ? 4 : 2;

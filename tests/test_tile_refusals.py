@@ -1,4 +1,4 @@
-"""Lists of shared prefixes that the C entry refuses before it launches anything: no GPU is needed."""
+"""Lists of shared prefixes, and block tables, that the C entry refuses before it launches anything: no GPU is needed."""
 import pytest
 
 from swifttransformer_amd.ops import kernels as K
@@ -22,3 +22,12 @@ def test_lists_that_are_whole():
 def test_lists_that_are_not(kw):
     """(The join looks for a row in the groups' lists: an empty one, or starts without groups, leave it nothing to look at.)"""
     assert call(**kw) != 0 and "lists" in K._lib().st_last_error().decode()
+
+
+@pytest.mark.parametrize("max_pages,page_size,fits", [((1 << 27) - 1, 16, False), ((1 << 31) - 2, 1, False), ((1 << 31) - 513, 1, True), ((1 << 27) - 32, 16, False),
+                                                      ((1 << 27) - 33, 16, True), ((1 << 27) - 31, 16, False), (1 << 20, 1 << 11, False)])
+def test_tables_whose_last_keys_are_close_to_what_an_int_holds(max_pages, page_size, fits):
+    """(A wave's next blocks of keys are looked up ahead, behind the last key too.)"""
+    kw = dict(ONE, max_pages=max_pages, page_size=page_size, page_stride=2 * page_size * 64 if page_size <= 16 else 1 << 30, exp_stride=2 * page_size)
+    rc = call(**kw)
+    assert (rc == 0) == fits and (fits or "2^31" in K._lib().st_last_error().decode())
