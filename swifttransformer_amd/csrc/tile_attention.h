@@ -283,7 +283,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
             s_sees[16 * rt + r16] = sees;
         }
         most = max(most, sees);
-        lim[rt] = t < 0 ? 0x7fffffff : sees;                // (a row that is none takes whatever comes)
+        lim[rt] = sees == 0 ? 0x7fffffff : sees;            // (a row that is none, or sees none, takes whatever comes)
         least = min(least, lim[rt]);
     }
     most = __builtin_amdgcn_readfirstlane(row16<true>(most));
@@ -442,7 +442,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                         x &= ~(n | none_of);
                     };
                     clear(v.x); clear(v.y); clear(v.z); clear(v.w);
-                    asm volatile("" : "+v"(odd));
+                    asm volatile("" : "+v"(odd));           // (chunk by chunk: all at once take a register each)
                 }
             }
             wild |= __any(odd != 0);
@@ -645,6 +645,11 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
     for (int v = 0; v < 4; ++v) top = max_raw(top, s_m[v * R + row]);
 #pragma unroll
     for (int v = 0; v < 4; ++v) sum += s_l[v * R + row] * weight_of(s_m[v * R + row], top, sl);
+    const bool any = s_sees[row] > 0;                       // (else zeros, and what its lanes hold is not looked at)
+    if (!any) {
+        top = kFloor;
+        sum = 0.f;
+    }
     // (a sum that is no number belongs to the result)
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t out_row = (int64_t)(w.slot >= 0 ? w.slot : t) * p.heads + head;
@@ -674,6 +679,7 @@ __device__ inline void tile_work(const StTileAttention& p, const TileWork& w, in
                     for (int r = 0; r < 4; ++r) o[r] += fabsf(x[r]) < INFINITY ? 0.f : x[r];
                 }
             }
+            if (!any) o = floatx4{0.f, 0.f, 0.f, 0.f};
             const float by = p.slots == 1 ? inverse : 1.f;
             const float res[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
             if (p.slots == 1)

@@ -155,3 +155,31 @@ def test_rows_with_a_prefix_that_no_group_lists(quant):
             kk, vv = pool.entries(table, t, lens[t])
             first = start[t] if t in left_out else 0
             compare(got[t], *reference(q[t], kk[first:], vv[first:], 4, 0.125))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_rows_that_see_nothing_beside_rows_that_see_all(hd, dtype, quant):
+    """Padding rows, and rows without a prefix, that a group lists: whatever their queries are, they get zeros (their own keys only), the others their results."""
+    g = torch.Generator().manual_seed(hd)
+    batch = shared_batch([(150, 9), (33, 4)], [20, 5, 1], 4, 2, hd, 16, dtype, quant, g)
+    pool, table, lens, start, shared, off, q = batch
+    k, v, ke, ve = pool.put()
+    n = len(lens)
+    item = list(range(n))
+    padding, plain = [shared[0], shared[4], shared[12]], shared[6]
+    for r in padding:
+        item[r] = -1
+        q[r] = math.nan
+    start = list(start)
+    start[plain] = 0
+    put = lambda x: ints(x).to(DEV)  # noqa: E731
+    for a, b in ((1, 1), (3, 2)):
+        got = K.attention_shared(q.to(DEV), k, v, put(item), put([m - 1 for m in lens]), table.to(DEV), 4, 0.125, put(start), put(shared), put(off), k_exp=ke,
+                                 v_exp=ve, shared_splits=a, own_splits=b)
+        for t in range(n):
+            if t in padding:
+                assert bool((got[t] == 0).all())
+            else:
+                compare(got[t], *reference(q[t], *pool.entries(table, t, lens[t]), 4, 0.125))
